@@ -191,6 +191,85 @@ int pi0_vision_profile_enable(pi0_vision_ctx* ctx, int on);
 int pi0_vision_profile_read(pi0_vision_ctx* ctx, int n_families, int64_t* launches,
                             double* total_ms);
 
+/* ---- text generation behind the prefix expert (no counterpart in the reference) ---------------
+ * Packed batches of requests over a key/value cache in pages of 8-bit codes: block tables and slot
+ * maps from request lengths, new tokens into the cache, attention of packed prompts, attention of
+ * one token per request over the cache. All context-free, all buffers the caller's, all int32
+ * arrays on the device. `err` (a device int, may be NULL) takes the first of pi0_paged_err and
+ * pi0_device_error's codes that a call meets and is left alone otherwise; what such a call wrote
+ * stays inside its buffers, and requests without a fault have their results.
+ *
+ * A page holds page_size tokens of one request. Token `pos` of request r lies in page
+ * block_table[r, pos / page_size] at row pos % page_size; its slot is page·page_size + row. */
+enum pi0_paged_err {
+  PI0_PAGED_ERR_LENGTH = 16, /* a length below zero, or more new tokens than num_tokens */
+  PI0_PAGED_ERR_TABLE = 17,  /* a request longer than its row of the block table */
+  PI0_PAGED_ERR_POOL = 18,   /* no free page left for a request */
+  PI0_PAGED_ERR_PAGE = 19    /* a page number outside the pool, or a slot that is not its token's */
+};
+
+/* Cache of one attention layer: codes [num_pages, kv_heads, page_size, head_dim] in e4m3, one fp32
+ * scale per page and kv head [num_pages, kv_heads]: the number is code·scale. head_dim a multiple
+ * of 8 up to 256, codes 16-byte aligned, num_pages·page_size below 2^31. */
+typedef struct pi0_kv8 {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int32_t num_pages, page_size, kv_heads, head_dim;
+} pi0_kv8;
+
+/* Requests with kv_lens[r] cached tokens take new_lens[r] more. New pages come from
+ * free_pages[*free_pos ...], in the order of the requests, and are written into block_table
+ * [batch, max_pages] (row stride table_stride) behind the pages that a request holds already.
+ * Writes cu_seqlens [batch + 1] (sums of new_lens), positions and slot_mapping [num_tokens] of the
+ * packed new tokens (-1 slots for tokens behind the last request's), kv_lens_out [batch] and
+ * free_pos_out [1], which may alias their inputs only if no other call reads these. A request that
+ * its table row or the pool cannot hold is not admitted: its slots are -1, its length stays.
+ * batch ≤ 16384. */
+int pi0_build_slots(int batch, const int32_t* kv_lens, const int32_t* new_lens,
+                    int32_t* block_table, int64_t table_stride, int max_pages,
+                    const int32_t* free_pages, int n_free, const int32_t* free_pos, int num_pages,
+                    int page_size, int num_tokens, int32_t* cu_seqlens, int32_t* positions,
+                    int32_t* slot_mapping, int32_t* kv_lens_out, int32_t* free_pos_out, int* err,
+                    pi0_stream_t stream);
+
+/* Keys and values [num_tokens, kv_heads, head_dim] (PI0_F16 / PI0_BF16; strides in elements,
+ * multiples of 8, last dimension contiguous, 16-byte aligned) into the cache at slot_mapping. The
+ * scale of a page and head is the smallest power of two, not below 2^-64, with which the largest
+ * magnitude of its tokens fits into ±448; tokens that join a page (kv_lens: tokens cached before)
+ * keep or raise its scale, and codes already there are rounded to a raised one. Infinities and NaN
+ * are stored as NaN and do not count for the scale. Tokens with slot -1 are left out. max_new: the
+ * most new tokens of one request, which sizes the launch (a larger request is still written). */
+int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                 const void* v, int64_t v_token_stride, int64_t v_head_stride, int num_tokens,
+                 int batch, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                 const int32_t* slot_mapping, int max_new, const pi0_kv8* cache, int* err,
+                 pi0_stream_t stream);
+
+/* Attention of packed prompts: request r has the queries cu_seqlens_q[r] .. cu_seqlens_q[r+1] of
+ * q [total_q, heads, head_dim] and the keys cu_seqlens_k[r] .. of k, v [total_k, kv_heads,
+ * head_dim] (strides and alignment as above); head h reads kv head h / (heads / kv_heads). Of Lq
+ * queries and Lk keys, query i sees key j if j ≤ i + Lk − Lq or j < prefix_lens[r] (NULL: 0,
+ * causal; Lk: every query sees every key). out [total_q, heads, head_dim] = softmax(scale·q·kᵀ)·v
+ * over the keys seen, fp32 softmax; a query that sees none, and a token of no request, give zeros.
+ * Keys and values that a query does not see do not reach its result, whatever they hold. */
+int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                         const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                         int total_q, int total_k, int heads, int kv_heads, int head_dim,
+                         int batch, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                         const int32_t* prefix_lens, float scale, void* out,
+                         int64_t o_token_stride, int64_t o_head_stride, int* err,
+                         pi0_stream_t stream);
+
+/* Attention of one token per request over the cache: q, out [batch, heads, head_dim]; the request
+ * sees its kv_lens[r] cached tokens (the new one's keys and values are written before the call).
+ * A request without any gives zeros. */
+int pi0_attention_paged(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                        int batch, int heads, const pi0_kv8* cache, const int32_t* block_table,
+                        int64_t table_stride, int max_pages, const int32_t* kv_lens, float scale,
+                        void* out, int64_t o_token_stride, int64_t o_head_stride, int* err,
+                        pi0_stream_t stream);
+
 /* ---- building block and measurement hooks (no counterpart in the reference) --------------- */
 
 /* y[M, N] = x[M, K] · w[N, K]^T in the context's model dtype (fp32 accumulation, one rounding):

@@ -1,0 +1,146 @@
+// The text-generation operators of include/pi0b200.h: block tables and slot maps, the 8-bit page
+// cache, attention over packed prompts and attention of single tokens over the cache. Context-free,
+// like pi0_embed_language: every buffer is the caller's, every call is asynchronous on the stream.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "pi0b200.h"
+#include "paged_slots.cuh"
+#include "paged_write.cuh"
+#include "paged_prompt.cuh"
+#include "paged_decode.cuh"
+
+using namespace pi0;
+using namespace pi0::paged;
+
+namespace {
+
+bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+bool dtype_ok(int dtype) { return dtype == PI0_F16 || dtype == PI0_BF16; }
+int launched() { return cudaGetLastError() == cudaSuccess ? PI0_OK : PI0_ERR_CUDA; }
+
+// one 16-bit operand [tokens, heads, head_dim]: 16-byte vectors along the last dimension
+bool rows_ok(const void* p, int64_t tok, int64_t head) {
+  return p && !off16(p) && tok > 0 && head > 0 && tok % 8 == 0 && head % 8 == 0;
+}
+
+bool cache_ok(const pi0_kv8* c) {
+  return c && c->k && c->v && c->k_scale && c->v_scale && !off16(c->k) && !off16(c->v) &&
+         c->num_pages >= 1 && c->page_size >= 1 && c->kv_heads >= 1 && c->head_dim >= 8 &&
+         c->head_dim % 8 == 0 && c->head_dim <= 256 &&
+         (int64_t)c->num_pages * c->page_size <= INT_MAX;
+}
+
+Cache cache_of(const pi0_kv8* c) {
+  return Cache{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale,
+               c->num_pages, c->page_size, c->kv_heads, c->head_dim};
+}
+
+}  // namespace
+
+extern "C" {
+
+int pi0_build_slots(int batch, const int32_t* kv_lens, const int32_t* new_lens,
+                    int32_t* block_table, int64_t table_stride, int max_pages,
+                    const int32_t* free_pages, int n_free, const int32_t* free_pos, int num_pages,
+                    int page_size, int num_tokens, int32_t* cu_seqlens, int32_t* positions,
+                    int32_t* slot_mapping, int32_t* kv_lens_out, int32_t* free_pos_out, int* err,
+                    pi0_stream_t stream) {
+  if (batch < 0 || max_pages < 1 || table_stride < max_pages || n_free < 0 || num_pages < 1 ||
+      page_size < 1 || num_tokens < 0 || (int64_t)num_pages * page_size > INT_MAX)
+    return PI0_ERR_INVALID;
+  if (!free_pos || !cu_seqlens || !free_pos_out || (n_free && !free_pages) ||
+      (batch && (!kv_lens || !new_lens || !block_table || !kv_lens_out)) ||
+      (num_tokens && (!positions || !slot_mapping)))
+    return PI0_ERR_INVALID;
+  if (batch > kSlotMaxBatch) return PI0_ERR_UNSUPPORTED;
+  const size_t smem = 2 * sizeof(int) * ((size_t)batch + 1);
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(build_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)smem) != cudaSuccess)
+    return PI0_ERR_CUDA;
+  SlotArgs a{kv_lens, new_lens, block_table, table_stride, free_pages, free_pos, cu_seqlens,
+             positions, slot_mapping, kv_lens_out, free_pos_out, err, batch, max_pages, n_free,
+             num_pages, page_size, num_tokens};
+  // two tokens a thread until one block per SM is reached
+  const int grid = std::max(1, std::min(148, (num_tokens + 2 * kSlotThreads - 1) / (2 * kSlotThreads)));
+  build_slots_kernel<<<grid, kSlotThreads, smem, stream>>>(a);
+  return launched();
+}
+
+int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                 const void* v, int64_t v_token_stride, int64_t v_head_stride, int num_tokens,
+                 int batch, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                 const int32_t* slot_mapping, int max_new, const pi0_kv8* cache, int* err,
+                 pi0_stream_t stream) {
+  if (!dtype_ok(dtype) || num_tokens < 0 || batch < 0 || max_new < 0 || !cache_ok(cache))
+    return PI0_ERR_INVALID;
+  if (num_tokens == 0 || batch == 0 || max_new == 0) return PI0_OK;
+  if (!rows_ok(k, k_token_stride, k_head_stride) || !rows_ok(v, v_token_stride, v_head_stride) ||
+      !cu_seqlens || !kv_lens || !slot_mapping)
+    return PI0_ERR_INVALID;
+  if (batch > 65535 || cache->kv_heads > 32767) return PI0_ERR_UNSUPPORTED;
+  WriteArgs a{{k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride},
+              cu_seqlens, kv_lens, slot_mapping, err, cache_of(cache), num_tokens};
+  // n tokens touch at most ⌈(n − 1)/page⌉ + 1 pages; a request with more than max_new loops
+  const int pages = (std::min(max_new, num_tokens) + cache->page_size - 2) / cache->page_size + 1;
+  const dim3 grid(pages, 2 * cache->kv_heads, batch);
+  if (dtype == PI0_F16) write_kv_kernel<__half><<<grid, kWriteThreads, 0, stream>>>(a);
+  else write_kv_kernel<__nv_bfloat16><<<grid, kWriteThreads, 0, stream>>>(a);
+  return launched();
+}
+
+int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                         const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                         int total_q, int total_k, int heads, int kv_heads, int head_dim,
+                         int batch, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                         const int32_t* prefix_lens, float scale, void* out,
+                         int64_t o_token_stride, int64_t o_head_stride, int* err,
+                         pi0_stream_t stream) {
+  if (!dtype_ok(dtype) || total_q < 0 || total_k < 0 || heads < 1 || kv_heads < 1 ||
+      heads % kv_heads || head_dim < 8 || head_dim % 8 || head_dim > 256 || batch < 0)
+    return PI0_ERR_INVALID;
+  if (total_q == 0) return PI0_OK;
+  if (batch == 0 || !cu_seqlens_q || !cu_seqlens_k || !rows_ok(q, q_token_stride, q_head_stride) ||
+      !rows_ok(out, o_token_stride, o_head_stride) ||
+      (total_k && (!rows_ok(k, k_token_stride, k_head_stride) ||
+                   !rows_ok(v, v_token_stride, v_head_stride))))
+    return PI0_ERR_INVALID;
+  const int64_t rows = (int64_t)total_q * heads;
+  if (rows > INT_MAX) return PI0_ERR_UNSUPPORTED;
+  PromptArgs a{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
+               v_token_stride, v_head_stride, o_token_stride, o_head_stride, cu_seqlens_q,
+               cu_seqlens_k, prefix_lens, err, scale * 1.4426950408889634f, batch, total_q, total_k,
+               heads, kv_heads, head_dim};
+  const unsigned grid = (unsigned)((rows + kRowWarps - 1) / kRowWarps);
+  if (dtype == PI0_F16) prompt_rows_kernel<__half><<<grid, 32 * kRowWarps, 0, stream>>>(a);
+  else prompt_rows_kernel<__nv_bfloat16><<<grid, 32 * kRowWarps, 0, stream>>>(a);
+  return launched();
+}
+
+int pi0_attention_paged(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                        int batch, int heads, const pi0_kv8* cache, const int32_t* block_table,
+                        int64_t table_stride, int max_pages, const int32_t* kv_lens, float scale,
+                        void* out, int64_t o_token_stride, int64_t o_head_stride, int* err,
+                        pi0_stream_t stream) {
+  if (!dtype_ok(dtype) || batch < 0 || heads < 1 || !cache_ok(cache) || heads % cache->kv_heads ||
+      max_pages < 1 || table_stride < max_pages)
+    return PI0_ERR_INVALID;
+  if (batch == 0) return PI0_OK;
+  if (!rows_ok(q, q_token_stride, q_head_stride) || !rows_ok(out, o_token_stride, o_head_stride) ||
+      !block_table || !kv_lens)
+    return PI0_ERR_INVALID;
+  if (batch > 65535) return PI0_ERR_UNSUPPORTED;
+  DecodeArgs a{q, out, q_token_stride, q_head_stride, o_token_stride, o_head_stride,
+               cache_of(cache), block_table, table_stride, kv_lens, err,
+               scale * 1.4426950408889634f, batch, heads, max_pages};
+  const dim3 grid(heads, batch);
+  if (dtype == PI0_F16) paged_rows_kernel<__half><<<grid, 32, 0, stream>>>(a);
+  else paged_rows_kernel<__nv_bfloat16><<<grid, 32, 0, stream>>>(a);
+  return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,184 @@
+// Block tables and slot maps from request lengths.
+//
+// With have = ⌈kv/page⌉ and need = ⌈(kv + new)/page⌉ − have, the new pages of request r are
+// free_pages[pos + Σ_{s<r} need_s ...]; token t of the packed batch belongs to the request with
+// cu[r] ≤ t < cu[r+1], has position kv_r + t − cu[r], and its slot is page·page_size + row.
+//
+// Bound by latency: two prefix sums over the requests, then independent lookups. Every block
+// repeats the sums (a few KB from L2) instead of waiting for another kernel that made them, so the
+// whole operator is one launch.
+#pragma once
+
+#include "paged_common.cuh"
+
+namespace pi0 {
+namespace paged {
+
+constexpr int kSlotThreads = 512;
+constexpr int kSlotMaxBatch = 16384;  // the two prefix sums live in shared memory (128 KB)
+
+struct SlotArgs {
+  const int* kv_lens;
+  const int* new_lens;
+  int* table;
+  int64_t table_stride;
+  const int* free_pages;
+  const int* free_pos;
+  int* cu;
+  int* positions;
+  int* slots;
+  int* kv_out;
+  int* free_pos_out;
+  int* err;
+  int batch, max_pages, n_free, num_pages, page_size, tokens;
+};
+
+// a + b for non-negative a, b, held at 2^31 − 1 (associative, so it can be scanned)
+__device__ __forceinline__ int add_sat(int a, int b) {
+  return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu);
+}
+
+// the last i in [0, n) with a[i] ≤ x, for ascending a with a[0] ≤ x
+__device__ __forceinline__ int last_le(const int* a, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
+  extern __shared__ int sm[];
+  int* s_cu = sm;                  // [batch + 1] tokens before request r
+  int* s_off = sm + a.batch + 1;   // [batch + 1] new pages before request r
+  __shared__ int s_warp[2][kSlotThreads / 32];
+  __shared__ int s_used;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int pos0 = max(0, *a.free_pos);
+  const int avail = max(0, a.n_free - pos0);
+  const int ps = a.page_size;
+  if (tid == 0) {
+    s_cu[0] = s_off[0] = 0;
+    s_used = 0;
+  }
+
+  // a request's own numbers; a length below zero counts as zero, and one that its table row cannot
+  // hold asks for no page
+  auto lens = [&](int r, int& kv, int& nw, int& have, int& need) -> int {
+    int code = 0;
+    kv = a.kv_lens[r];
+    nw = a.new_lens[r];
+    if (kv < 0 || nw < 0) code = PI0_PAGED_ERR_LENGTH;
+    kv = max(kv, 0);
+    nw = max(nw, 0);
+    const int64_t end = (int64_t)kv + nw;
+    have = (int)(((int64_t)kv + ps - 1) / ps);
+    need = 0;
+    if (end > (int64_t)a.max_pages * ps) code = PI0_PAGED_ERR_TABLE;
+    else need = (int)((end + ps - 1) / ps) - have;
+    return code;
+  };
+
+  int carry_c = 0, carry_o = 0;
+  for (int base = 0; base < a.batch; base += kSlotThreads) {
+    const int r = base + tid;
+    int kv = 0, nw = 0, have = 0, need = 0;
+    if (r < a.batch) {
+      const int code = lens(r, kv, nw, have, need);
+      if (code && blockIdx.x == 0) set_err(a.err, code);
+    }
+    int c = nw, o = need;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int pc = __shfl_up_sync(~0u, c, d), po = __shfl_up_sync(~0u, o, d);
+      if (lane >= d) {
+        c = add_sat(c, pc);
+        o = add_sat(o, po);
+      }
+    }
+    if (lane == 31) {
+      s_warp[0][warp] = c;
+      s_warp[1][warp] = o;
+    }
+    __syncthreads();
+    int bc = carry_c, bo = carry_o, tc = carry_c, to = carry_o;
+#pragma unroll
+    for (int w = 0; w < kSlotThreads / 32; ++w) {
+      if (w == warp) {
+        bc = tc;
+        bo = to;
+      }
+      tc = add_sat(tc, s_warp[0][w]);
+      to = add_sat(to, s_warp[1][w]);
+    }
+    if (r < a.batch) {
+      s_cu[r + 1] = add_sat(bc, c);
+      s_off[r + 1] = add_sat(bo, o);
+    }
+    carry_c = tc;
+    carry_o = to;
+    __syncthreads();
+  }
+
+  // admitted: the table row holds it and the pool has its pages. Offsets ascend, so of the
+  // requests that need pages the admitted ones are the first ones.
+  auto admitted = [&](int r, int kv, int nw) -> bool {
+    return (int64_t)kv + nw <= (int64_t)a.max_pages * ps &&
+           (s_off[r + 1] == s_off[r] || s_off[r + 1] <= avail);
+  };
+  if (blockIdx.x == 0) {
+    int used = 0;
+    bool short_of = false;
+    for (int r = tid; r <= a.batch; r += kSlotThreads) a.cu[r] = s_cu[r];
+    for (int r = tid; r < a.batch; r += kSlotThreads) {
+      const int kv = max(a.kv_lens[r], 0), nw = max(a.new_lens[r], 0);
+      const bool ok = admitted(r, kv, nw);
+      a.kv_out[r] = ok ? kv + nw : kv;
+      if (s_off[r + 1] > s_off[r]) {
+        if (ok) used = max(used, s_off[r + 1]);
+        else short_of = true;
+      }
+    }
+    if (used) atomicMax(&s_used, used);
+    if (short_of) set_err(a.err, PI0_PAGED_ERR_POOL);
+    if (tid == 0 && s_cu[a.batch] > a.tokens) set_err(a.err, PI0_PAGED_ERR_LENGTH);
+    __syncthreads();
+    if (tid == 0) *a.free_pos_out = pos0 + s_used;
+  }
+
+  const int g = blockIdx.x * kSlotThreads + tid, step = gridDim.x * kSlotThreads;
+  // page i of the new ones
+  const int total = min(s_off[a.batch], avail);
+  for (int i = g; i < total; i += step) {
+    const int r = last_le(s_off, a.batch, i);
+    if (s_off[r + 1] > avail) continue;  // not admitted
+    const int have = (int)(((int64_t)max(a.kv_lens[r], 0) + ps - 1) / ps);
+    const int page = a.free_pages[pos0 + i];
+    if ((unsigned)page >= (unsigned)a.num_pages) set_err(a.err, PI0_PAGED_ERR_PAGE);
+    a.table[(int64_t)r * a.table_stride + have + (i - s_off[r])] = page;
+  }
+  for (int t = g; t < a.tokens; t += step) {
+    int pos = 0, slot = -1;
+    if (t < s_cu[a.batch]) {
+      const int r = last_le(s_cu, a.batch, t);
+      const int kv = max(a.kv_lens[r], 0), nw = max(a.new_lens[r], 0);
+      const int have = (int)(((int64_t)kv + ps - 1) / ps);
+      pos = kv + (t - s_cu[r]);
+      if (admitted(r, kv, nw)) {
+        const int col = pos / ps;
+        // a page that the request holds already stands in its table row; a new one is read from
+        // the free list, so no thread waits for another's table write
+        const int page = col < have ? a.table[(int64_t)r * a.table_stride + col]
+                                    : a.free_pages[pos0 + s_off[r] + (col - have)];
+        if ((unsigned)page < (unsigned)a.num_pages) slot = page * ps + pos % ps;
+        else set_err(a.err, PI0_PAGED_ERR_PAGE);
+      }
+    }
+    a.positions[t] = pos;
+    a.slots[t] = slot;
+  }
+}
+
+}  // namespace paged
+}  // namespace pi0

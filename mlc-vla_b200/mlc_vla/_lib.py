@@ -1,7 +1,8 @@
 """Build and load ``libpi0b200.so`` (the sm_100a kernels behind include/pi0b200.h).
 
-``build()`` compiles ``csrc/pi0_api.cu`` in-tree with nvcc for ``sm_100a``; ``load()`` opens the
-library with ctypes and declares every entry point of the header. There is no fallback: when
+``build()`` compiles ``csrc/pi0_api.cu`` (the model path) and ``csrc/paged_api.cu`` (the
+text-generation operators) side by side in-tree with nvcc for ``sm_100a`` and links them;
+``load()`` opens the library with ctypes and declares every entry point of the header. There is no fallback: when
 the library is missing, ``load()`` raises.
 """
 
@@ -21,8 +22,9 @@ LIB_PATH = os.path.join(PKG_DIR, "lib", "libpi0b200.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
+UNITS = ("pi0_api.cu", "paged_api.cu")
 
 PI0_OK, PI0_ERR_INVALID, PI0_ERR_CUDA, PI0_ERR_NO_PARAMS, PI0_ERR_DEVICE, PI0_ERR_UNSUPPORTED = range(6)
 PI0_F16, PI0_BF16, PI0_F32, PI0_U32 = range(4)
@@ -43,6 +45,7 @@ EXPORTED = (
     "pi0_vision_param_info", "pi0_vision_set_params", "pi0_embed_image",
     "pi0_vision_launch_count", "pi0_vision_device_error", "pi0_vision_profile_enable",
     "pi0_vision_profile_read",
+    "pi0_build_slots", "pi0_write_kv", "pi0_attention_prompt", "pi0_attention_paged",
 )
 
 
@@ -51,11 +54,23 @@ def _sources():
             if f.endswith((".cu", ".cuh", ".h"))] + [os.path.join(INCLUDE_DIR, "pi0b200.h")]
 
 
+def _unit_sources(unit: str):
+    """The sources that an object file is older than when it has to be compiled again: the
+    paged_* files go into paged_api.cu only, which needs two of the others."""
+    paged = unit.startswith("paged_")
+    shared = ("common.cuh", "gemm_tc.cuh", "pi0b200.h")
+    return [s for s in _sources()
+            if os.path.basename(s) in shared
+            or os.path.basename(s).startswith("paged_") == paged]
+
+
+def _stale(target: str, sources) -> bool:
+    return not os.path.exists(target) or any(os.path.getmtime(s) > os.path.getmtime(target)
+                                             for s in sources)
+
+
 def needs_build() -> bool:
-    if not os.path.exists(LIB_PATH):
-        return True
-    t = os.path.getmtime(LIB_PATH)
-    return any(os.path.getmtime(s) > t for s in _sources())
+    return _stale(LIB_PATH, _sources())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -63,8 +78,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB_PATH
     os.makedirs(os.path.dirname(LIB_PATH), exist_ok=True)
+    objects, running = [], []
+    for unit in UNITS:
+        obj = os.path.join(os.path.dirname(LIB_PATH), unit.replace(".cu", ".o"))
+        objects.append(obj)
+        if force or _stale(obj, _unit_sources(unit)):
+            cmd = ["nvcc", *NVCC_FLAGS, f"-I{INCLUDE_DIR}", "-c", os.path.join(CSRC_DIR, unit),
+                   "-o", obj + ".tmp"]
+            if verbose:
+                print(" ".join(cmd))
+            running.append((obj, cmd, subprocess.Popen(cmd, cwd=CSRC_DIR)))
+    failed = [cmd for _, cmd, p in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    for obj, _, _ in running:
+        os.replace(obj + ".tmp", obj)
     tmp = LIB_PATH + ".tmp"
-    cmd = ["nvcc", *NVCC_FLAGS, f"-I{INCLUDE_DIR}", os.path.join(CSRC_DIR, "pi0_api.cu"), "-o", tmp]
+    cmd = ["nvcc", *NVCC_FLAGS, "-shared", *objects, "-o", tmp]
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True, cwd=CSRC_DIR)
@@ -98,6 +128,17 @@ class Pi0VisionConfigC(ctypes.Structure):
         ("num_attention_heads", ctypes.c_int32), ("projection_dim", ctypes.c_int32),
         ("dtype", ctypes.c_int32), ("max_images", ctypes.c_int32),
         ("layer_norm_eps", ctypes.c_float),
+    ]
+
+
+class Pi0Kv8C(ctypes.Structure):
+    """Mirror of ``struct pi0_kv8`` (include/pi0b200.h)."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
     ]
 
 
@@ -160,6 +201,16 @@ def load():
         lib.pi0_vision_device_error.argtypes = [vp]
         lib.pi0_vision_profile_enable.argtypes = [vp, i32]
         lib.pi0_vision_profile_read.argtypes = lib.pi0_profile_read.argtypes
+        kv8, f32 = ctypes.POINTER(Pi0Kv8C), ctypes.c_float
+        lib.pi0_build_slots.argtypes = [i32, vp, vp, vp, i64, i32, vp, i32, vp, i32, i32, i32, vp,
+                                        vp, vp, vp, vp, vp, vp]
+        lib.pi0_write_kv.argtypes = [i32, vp, i64, i64, vp, i64, i64, i32, i32, vp, vp, vp, i32,
+                                     kv8, vp, vp]
+        lib.pi0_attention_prompt.argtypes = [i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, i32,
+                                             i32, i32, i32, i32, i32, vp, vp, vp, f32, vp, i64,
+                                             i64, vp, vp]
+        lib.pi0_attention_paged.argtypes = [i32, vp, i64, i64, i32, i32, kv8, vp, i64, i32, vp,
+                                            f32, vp, i64, i64, vp, vp]
         for name in EXPORTED:
             getattr(lib, name).restype = getattr(lib, name).restype or ctypes.c_int
         lib.pi0_last_error.restype = ctypes.c_char_p
