@@ -263,12 +263,18 @@ int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64
 
 /* Attention of one token per request over the cache: q, out [batch, heads, head_dim]; the request
  * sees its kv_lens[r] cached tokens (the new one's keys and values are written before the call).
- * A request without any gives zeros. */
+ * A request without any gives zeros. workspace (16-byte aligned, of the size that
+ * pi0_attention_paged_workspace returns for the current device; -1: bad sizes or no device) holds
+ * what the parts of a request's tokens add up to until they are joined: its contents before and
+ * after a call do not matter, but calls that may run at the same time need one each. Head sizes 64,
+ * 128 and 256 on pages of 8, 16, 32 or 64 tokens or of whole 128s run on tensor cores and need
+ * `err`, which also takes the codes of bounded waits; the others need neither. */
+int64_t pi0_attention_paged_workspace(int heads, int kv_heads, int head_dim, int page_size);
 int pi0_attention_paged(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                         int batch, int heads, const pi0_kv8* cache, const int32_t* block_table,
                         int64_t table_stride, int max_pages, const int32_t* kv_lens, float scale,
-                        void* out, int64_t o_token_stride, int64_t o_head_stride, int* err,
-                        pi0_stream_t stream);
+                        void* out, int64_t o_token_stride, int64_t o_head_stride, void* workspace,
+                        int64_t workspace_bytes, int* err, pi0_stream_t stream);
 
 /* ---- building block and measurement hooks (no counterpart in the reference) --------------- */
 

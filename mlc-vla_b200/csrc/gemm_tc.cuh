@@ -65,7 +65,7 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
 // soon as another role has reported an error (unless `bail` is false: drain waits). The hot
 // loop only polls the barrier; the clock is read every 128 polls and the (global) error flag
 // every 8192, so a completed phase is seen without a memory round trip in the way.
-__device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, int* err, int code,
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, int* err, int code,
                                             bool bail) {
   const unsigned long long t0 = globaltimer();
   for (uint32_t it = 1;; ++it) {

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "pi0b200.h"
@@ -36,6 +37,127 @@ bool cache_ok(const pi0_kv8* c) {
 Cache cache_of(const pi0_kv8* c) {
   return Cache{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale,
                c->num_pages, c->page_size, c->kv_heads, c->head_dim};
+}
+
+constexpr int kMaxDevices = 64;
+
+// SMs of the current device (0: the runtime failed)
+int sm_count(int* device) {
+  static std::atomic<int> known[kMaxDevices];
+  if (cudaGetDevice(device) != cudaSuccess || *device < 0 || *device >= kMaxDevices) return 0;
+  int n = known[*device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *device) != cudaSuccess) return 0;
+    known[*device].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// lets kernel F use `bytes` of dynamic shared memory, once per device
+template <auto F>
+bool allow_smem(int device, int bytes) {
+  static std::atomic<bool> done[kMaxDevices];
+  if (done[device].load(std::memory_order_relaxed)) return true;
+  if (cudaFuncSetAttribute(F, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return false;
+  done[device].store(true, std::memory_order_relaxed);
+  return true;
+}
+
+// ---- TMA tensor maps (driver entry point fetched through the runtime, no libcuda link) ------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static std::atomic<EncodeTiledFn> known{nullptr};
+  EncodeTiledFn f = known.load(std::memory_order_acquire);
+  if (f) return f;
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+      q != cudaDriverEntryPointSuccess)
+    return nullptr;
+  f = reinterpret_cast<EncodeTiledFn>(fn);
+  known.store(f, std::memory_order_release);
+  return f;
+}
+
+// Map of `rank` dimensions, innermost first; strides in bytes of the dimensions behind it. Out of
+// bounds reads as zero. Swizzled over `span` bytes, the width of a box.
+template <int RANK>
+int make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, const cuuint64_t (&dims)[RANK],
+             const cuuint64_t (&strides)[RANK - 1], const cuuint32_t (&box)[RANK], int span) {
+  const EncodeTiledFn f = encode_fn();
+  if (!f) return PI0_ERR_CUDA;
+  cuuint32_t ones[RANK];
+  for (auto& o : ones) o = 1;
+  const CUresult r = f(m, type, RANK, const_cast<void*>(base), dims, strides, box, ones,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       span == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PI0_OK : PI0_ERR_CUDA;
+}
+
+// ---- attention over the cache ---------------------------------------------------------------
+
+// Whether the tensor-core form takes these sizes: a head fills whole swizzle rows, a page divides a
+// tile of 128 keys into boxes of whole 8-row groups or is made of whole tiles.
+bool paged_tc(int head_dim, int page_size, int64_t planes) {
+  return (head_dim == 64 || head_dim == 128 || head_dim == 256) &&
+         (page_size % 128 == 0 || (page_size % 8 == 0 && 128 % page_size == 0)) && planes <= INT_MAX;
+}
+
+// heads of a unit's columns: 8 cover most groups; wider groups go 16 at a time
+int paged_heads(int heads, int kv_heads) { return heads / kv_heads <= 8 ? 8 : 16; }
+
+template <int HD, int NH>
+int64_t paged_ws(int sms) {
+  using C = DecCfg<HD, NH>;
+  return (int64_t)sms * C::OCC * (16 + 2 * C::PARTIAL * (int64_t)sizeof(float));
+}
+
+template <typename T, int HD, int NH>
+int run_paged(const DecodeArgs& a, int device, int sms, cudaStream_t st) {
+  using C = DecCfg<HD, NH>;
+  const Cache& c = a.cache;
+  CUtensorMap tk, tv;
+  const cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)c.page_size,
+                              (cuuint64_t)c.num_pages * c.kv_heads};
+  const cuuint64_t strides[2] = {(cuuint64_t)HD, (cuuint64_t)HD * c.page_size};
+  const cuuint32_t box[3] = {(cuuint32_t)C::ROW, (cuuint32_t)std::min(c.page_size, kDecTile), 1};
+  int rc = make_map<3>(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.k, dims, strides, box, C::ROW);
+  if (!rc) rc = make_map<3>(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.v, dims, strides, box, C::ROW);
+  if (rc) return rc;
+  if (!allow_smem<paged_decode_kernel<T, HD, NH>>(device, C::SMEM)) return PI0_ERR_CUDA;
+  const int group = a.heads / c.kv_heads;
+  const int64_t most = (int64_t)a.batch * c.kv_heads * ((group + NH - 1) / NH) *
+                       (((int64_t)a.max_pages * c.page_size + kDecTile - 1) / kDecTile);
+  const int ctas = (int)std::min<int64_t>((int64_t)sms * C::OCC, most);
+  paged_decode_kernel<T, HD, NH><<<ctas, kDecThreads, C::SMEM, st>>>(tk, tv, a);
+  if (cudaGetLastError() != cudaSuccess) return PI0_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, std::min(NH, group));
+  cfg.blockDim = dim3(HD);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, HD, NH>, a, ctas) == cudaSuccess
+             ? PI0_OK : PI0_ERR_CUDA;
+}
+
+template <typename T>
+int run_paged_any(const DecodeArgs& a, int device, int sms, cudaStream_t st) {
+  const bool wide = paged_heads(a.heads, a.cache.kv_heads) == 16;
+  switch (a.cache.head_dim) {
+    case 64: return wide ? run_paged<T, 64, 16>(a, device, sms, st) : run_paged<T, 64, 8>(a, device, sms, st);
+    case 128: return wide ? run_paged<T, 128, 16>(a, device, sms, st) : run_paged<T, 128, 8>(a, device, sms, st);
+    default: return wide ? run_paged<T, 256, 16>(a, device, sms, st) : run_paged<T, 256, 8>(a, device, sms, st);
+  }
 }
 
 }  // namespace
@@ -121,11 +243,25 @@ int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64
   return launched();
 }
 
+int64_t pi0_attention_paged_workspace(int heads, int kv_heads, int head_dim, int page_size) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || page_size < 1) return -1;
+  if (!paged_tc(head_dim, page_size, 1)) return 0;
+  int device;
+  const int sms = sm_count(&device);
+  if (!sms) return -1;
+  const bool wide = paged_heads(heads, kv_heads) == 16;
+  switch (head_dim) {
+    case 64: return wide ? paged_ws<64, 16>(sms) : paged_ws<64, 8>(sms);
+    case 128: return wide ? paged_ws<128, 16>(sms) : paged_ws<128, 8>(sms);
+    default: return wide ? paged_ws<256, 16>(sms) : paged_ws<256, 8>(sms);
+  }
+}
+
 int pi0_attention_paged(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                         int batch, int heads, const pi0_kv8* cache, const int32_t* block_table,
                         int64_t table_stride, int max_pages, const int32_t* kv_lens, float scale,
-                        void* out, int64_t o_token_stride, int64_t o_head_stride, int* err,
-                        pi0_stream_t stream) {
+                        void* out, int64_t o_token_stride, int64_t o_head_stride, void* workspace,
+                        int64_t workspace_bytes, int* err, pi0_stream_t stream) {
   if (!dtype_ok(dtype) || batch < 0 || heads < 1 || !cache_ok(cache) || heads % cache->kv_heads ||
       max_pages < 1 || table_stride < max_pages)
     return PI0_ERR_INVALID;
@@ -136,7 +272,17 @@ int pi0_attention_paged(int dtype, const void* q, int64_t q_token_stride, int64_
   if (batch > 65535) return PI0_ERR_UNSUPPORTED;
   DecodeArgs a{q, out, q_token_stride, q_head_stride, o_token_stride, o_head_stride,
                cache_of(cache), block_table, table_stride, kv_lens, err,
-               scale * 1.4426950408889634f, batch, heads, max_pages};
+               static_cast<float*>(workspace), scale * 1.4426950408889634f, batch, heads, max_pages};
+  if (paged_tc(cache->head_dim, cache->page_size, (int64_t)cache->num_pages * cache->kv_heads)) {
+    const int64_t need = pi0_attention_paged_workspace(heads, cache->kv_heads, cache->head_dim,
+                                                       cache->page_size);
+    if (need < 0) return PI0_ERR_CUDA;
+    if (!workspace || off16(workspace) || workspace_bytes < need || !err) return PI0_ERR_INVALID;
+    int device;
+    const int sms = sm_count(&device);
+    return dtype == PI0_F16 ? run_paged_any<__half>(a, device, sms, stream)
+                            : run_paged_any<__nv_bfloat16>(a, device, sms, stream);
+  }
   const dim3 grid(heads, batch);
   if (dtype == PI0_F16) paged_rows_kernel<__half><<<grid, 32, 0, stream>>>(a);
   else paged_rows_kernel<__nv_bfloat16><<<grid, 32, 0, stream>>>(a);

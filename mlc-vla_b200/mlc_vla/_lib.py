@@ -46,6 +46,7 @@ EXPORTED = (
     "pi0_vision_launch_count", "pi0_vision_device_error", "pi0_vision_profile_enable",
     "pi0_vision_profile_read",
     "pi0_build_slots", "pi0_write_kv", "pi0_attention_prompt", "pi0_attention_paged",
+    "pi0_attention_paged_workspace",
 )
 
 
@@ -210,7 +211,9 @@ def load():
                                              i32, i32, i32, i32, i32, vp, vp, vp, f32, vp, i64,
                                              i64, vp, vp]
         lib.pi0_attention_paged.argtypes = [i32, vp, i64, i64, i32, i32, kv8, vp, i64, i32, vp,
-                                            f32, vp, i64, i64, vp, vp]
+                                            f32, vp, i64, i64, vp, i64, vp, vp]
+        lib.pi0_attention_paged_workspace.argtypes = [i32, i32, i32, i32]
+        lib.pi0_attention_paged_workspace.restype = ctypes.c_int64
         for name in EXPORTED:
             getattr(lib, name).restype = getattr(lib, name).restype or ctypes.c_int
         lib.pi0_last_error.restype = ctypes.c_char_p

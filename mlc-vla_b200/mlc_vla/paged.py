@@ -19,6 +19,7 @@ device int32 tensor of one element, or, where none is given, in a flag of the de
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Dict, NamedTuple, Optional
 
@@ -72,7 +73,11 @@ _flags: Dict[int, torch.Tensor] = {}
 def _flag(device: torch.device) -> torch.Tensor:
     f = _flags.get(device.index)
     if f is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the device's error flag does not exist yet: make one call before "
+                               "the capture, or give `err`")
         f = _flags[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.synchronize(device)  # zero before any stream's kernel may write it
     return f
 
 
@@ -168,6 +173,15 @@ def _call(name: str, device: torch.device, *args) -> None:
             rc = getattr(lib, name)(*args, _stream(device))
     if rc:
         _lib.check(rc, None, name)
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(device: torch.device, heads: int, kv_heads: int, dim: int, page: int) -> int:
+    with torch.cuda.device(device):
+        n = _lib.load().pi0_attention_paged_workspace(heads, kv_heads, dim, page)
+    if n < 0:
+        raise _lib.Pi0Error(_lib.PI0_ERR_CUDA, "pi0_attention_paged_workspace")
+    return n
 
 
 def build_slots(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
@@ -314,10 +328,12 @@ def attention_paged(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor,
     else:
         _rows(out, "out", dev, q.dtype, q.shape)
     max_pages = block_table.shape[1]
+    ws = torch.empty(_workspace_bytes(dev, heads, c.kv_heads, dim, c.page_size), dtype=torch.uint8,
+                     device=dev)
     _call("pi0_attention_paged", dev, code, q.data_ptr(), *_strides(q), batch, heads,
           ctypes.byref(c), block_table.data_ptr(), max(block_table.stride(0), max_pages),
           max_pages, kv_lens.data_ptr(), 1.0 / math.sqrt(dim) if scale is None else scale,
-          out.data_ptr(), *_strides(out), _err_ptr(err, dev))
+          out.data_ptr(), *_strides(out), ws.data_ptr(), ws.numel(), _err_ptr(err, dev))
     return out
 
 

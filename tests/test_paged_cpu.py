@@ -67,7 +67,7 @@ def test_c_entry_points_refuse():
 
     def decode(dtype=0, q=one, heads=8, c=ctypes.byref(kv), table=one, stride=4, columns=4, batch=1):
         return lib.pi0_attention_paged(dtype, q, 512, 64, batch, heads, c, table, stride, columns, one,
-                                       0.125, one, 512, 64, None, None)
+                                       0.125, one, 512, 64, None, 0, None, None)
 
     assert [decode(dtype=2), decode(q=None), decode(heads=7), decode(c=None), decode(table=None),
             decode(stride=3), decode(columns=0), decode(batch=-1)] == [bad] * 8
