@@ -251,7 +251,9 @@ int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_hea
  * queries and Lk keys, query i sees key j if j ≤ i + Lk − Lq or j < prefix_lens[r] (NULL: 0,
  * causal; Lk: every query sees every key). out [total_q, heads, head_dim] = softmax(scale·q·kᵀ)·v
  * over the keys seen, fp32 softmax; a query that sees none, and a token of no request, give zeros.
- * Keys and values that a query does not see do not reach its result, whatever they hold. */
+ * Keys and values that a query does not see do not reach its result, whatever they hold. Head
+ * sizes 64, 128 and 256 with up to 128 query heads per kv head run on tensor cores and need `err`,
+ * which also takes the codes of bounded waits; the others need none. */
 int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const void* k, int64_t k_token_stride, int64_t k_head_stride,
                          const void* v, int64_t v_token_stride, int64_t v_head_stride,

@@ -100,6 +100,45 @@ int make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, const c
   return r == CUDA_SUCCESS ? PI0_OK : PI0_ERR_CUDA;
 }
 
+// ---- attention over prompts -----------------------------------------------------------------
+
+template <typename T, int HD>
+int run_prompt(const PromptArgs& a, int device, cudaStream_t st) {
+  using C = PromptCfg<HD>;
+  constexpr CUtensorMapDataType type =
+      Tr<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  // a tile's 128 rows are the group's heads of as many tokens as fit
+  const int group = a.heads / a.kv_heads, tok = 128 / group;
+  auto map = [&](CUtensorMap* m, const void* p, int heads, int total, int64_t head_stride,
+                 int64_t token_stride, int box_heads, int box_tokens) {
+    const cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)heads, (cuuint64_t)total};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+    return make_map<3>(m, type, p, dims, strides, box, 128);
+  };
+  CUtensorMap tq, tk, tv;
+  int rc = map(&tq, a.q, a.heads, a.total_q, a.q_head, a.q_tok, group, tok);
+  if (!rc) rc = map(&tk, a.k, a.kv_heads, a.total_k, a.k_head, a.k_tok, 1, kKeys);
+  if (!rc) rc = map(&tv, a.v, a.kv_heads, a.total_k, a.v_head, a.v_tok, 1, C::VKEYS);
+  if (rc) return rc;
+  if (!allow_smem<prompt_tc_kernel<T, HD>>(device, C::SMEM)) return PI0_ERR_CUDA;
+  // every request has at most one tile that is not full
+  const int64_t tiles = (int64_t)a.total_q / (C::NQ * tok) + a.batch;
+  const int64_t grid = tiles * a.kv_heads;
+  if (grid > INT_MAX) return PI0_ERR_UNSUPPORTED;
+  prompt_tc_kernel<T, HD><<<(unsigned)grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, a, tok);
+  return launched();
+}
+
+template <typename T>
+int run_prompt_any(const PromptArgs& a, int device, cudaStream_t st) {
+  switch (a.head_dim) {
+    case 64: return run_prompt<T, 64>(a, device, st);
+    case 128: return run_prompt<T, 128>(a, device, st);
+    default: return run_prompt<T, 256>(a, device, st);
+  }
+}
+
 // ---- attention over the cache ---------------------------------------------------------------
 
 // Whether the tensor-core form takes these sizes: a head fills whole swizzle rows, a page divides a
@@ -237,6 +276,14 @@ int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64
                v_token_stride, v_head_stride, o_token_stride, o_head_stride, cu_seqlens_q,
                cu_seqlens_k, prefix_lens, err, scale * 1.4426950408889634f, batch, total_q, total_k,
                heads, kv_heads, head_dim};
+  if ((head_dim == 64 || head_dim == 128 || head_dim == 256) && heads / kv_heads <= 128 &&
+      total_k > 0) {
+    int device;
+    if (!err) return PI0_ERR_INVALID;
+    if (!sm_count(&device)) return PI0_ERR_CUDA;
+    return dtype == PI0_F16 ? run_prompt_any<__half>(a, device, stream)
+                            : run_prompt_any<__nv_bfloat16>(a, device, stream);
+  }
   const unsigned grid = (unsigned)((rows + kRowWarps - 1) / kRowWarps);
   if (dtype == PI0_F16) prompt_rows_kernel<__half><<<grid, 32 * kRowWarps, 0, stream>>>(a);
   else prompt_rows_kernel<__nv_bfloat16><<<grid, 32 * kRowWarps, 0, stream>>>(a);

@@ -5,6 +5,7 @@
 #pragma once
 
 #include "paged_common.cuh"
+#include "paged_tc.cuh"
 
 namespace pi0 {
 namespace paged {
@@ -74,6 +75,488 @@ __global__ void __launch_bounds__(32 * kRowWarps) prompt_rows_kernel(PromptArgs 
                        a.v_tok};
   attend_row(reinterpret_cast<const T*>(a.q) + t * a.q_tok + h * a.q_head, a.head_dim, n, a.c, kv,
              out);
+}
+
+// ---- tensor-core form -----------------------------------------------------------------------------
+
+constexpr int kKeys = 128;             // keys per tile
+constexpr float kPromptGrow = 8.f;     // the reference maximum is raised when it would grow by 2^8
+
+template <int HD>
+struct PromptCfg {
+  static constexpr int NQ = HD == 256 ? 1 : 2;      // tiles of 128 query rows per CTA
+  static constexpr int SPT = HD == 256 ? 2 : 1;     // ring slots per K or V tile
+  static constexpr int SLOT = kKeys * HD * 2 / SPT;
+  static constexpr int SLOTS = HD == 64 ? 8 : 5;
+  static constexpr int Q_TILE = 128 * HD * 2;
+  static constexpr int SMEM = NQ * Q_TILE + SLOTS * SLOT + 1024;
+  static constexpr int THREADS = 64 + NQ * 128;    // producer, MMA; softmax
+  static constexpr int VKEYS = kKeys / SPT;         // keys of a V slot
+  // tensor memory: two tiles of logits, each overlaid by its weights, then the sums
+  static constexpr int O_COL = 256;
+};
+
+struct PromptTile {
+  int q0, lq, k0, lk, prefix, t0;
+};
+
+// largest of 32 logits, in four chains
+__device__ __forceinline__ float max32(const float (&s)[32]) {
+  float a = s[0], b = s[1], c = s[2], d = s[3];
+#pragma unroll
+  for (int j = 4; j < 32; j += 4) {
+    a = fmaxf(a, s[j]);
+    b = fmaxf(b, s[j + 1]);
+    c = fmaxf(c, s[j + 2]);
+    d = fmaxf(d, s[j + 3]);
+  }
+  return fmaxf(fmaxf(a, b), fmaxf(c, d));
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
+    prompt_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
+                     const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, PromptArgs a, int tok) {
+  using C = PromptCfg<HD>;
+  constexpr int NQ = C::NQ, SPT = C::SPT, SLOTS = C::SLOTS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = base + SLOTS * C::SLOT;
+  __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, s_full[2], p_full[2],
+      pv_done[2], drain;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_scan[C::THREADS / 32], s_req, s_tile, s_bad;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kv = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
+  const int group = a.heads / a.kv_heads;
+
+  if (tid == 0) {
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(&drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    s_req = -1;
+    s_bad = 0x7fffffff;
+  }
+  // ---- which tile: the tiles of the requests are numbered in order; `index` lies in one of them
+  const int span = NQ * tok;
+  {
+    const int per = (a.batch + C::THREADS - 1) / C::THREADS;
+    const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+    int mine = 0, t0, n;
+    for (int b = b0; b < b1; ++b) {
+      seq_span(a.cu_q, b, a.total_q, t0, n);
+      mine += (n + span - 1) / span;
+    }
+    int inc = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(~0u, inc, d);
+      if (lane >= d) inc += up;
+    }
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    int before = inc - mine;
+#pragma unroll
+    for (int w = 0; w < C::THREADS / 32; ++w)
+      if (w < warp) before += s_scan[w];
+    if (index >= before && index < before + mine) {
+      int x = index - before;
+      for (int b = b0;; ++b) {
+        seq_span(a.cu_q, b, a.total_q, t0, n);
+        const int nt = (n + span - 1) / span;
+        if (x < nt) {
+          s_req = b;
+          s_tile = nt - 1 - x;  // the last tile of a request sees the most keys: first
+          break;
+        }
+        x -= nt;
+      }
+    }
+    // tokens of no request: zeros
+    if (index == 0 && kv == 0) {
+      const int first = min(max(a.cu_q[0], 0), a.total_q);
+      const int behind = min(max(a.cu_q[a.batch], first), a.total_q);
+      const int64_t none = (int64_t)(first + a.total_q - behind) * a.heads * (HD / 8);
+      for (int64_t i = tid; i < none; i += C::THREADS) {
+        const int64_t row = i / (HD / 8);
+        int t = (int)(row / a.heads);
+        t = t < first ? t : behind + t - first;
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + t * a.o_tok +
+                                  (row % a.heads) * a.o_head + (i % (HD / 8)) * 8) =
+            make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  __syncthreads();
+  if (s_req < 0) return;  // the grid is an upper bound of the tiles
+  PromptTile p;
+  seq_span(a.cu_q, s_req, a.total_q, p.q0, p.lq);
+  seq_span(a.cu_k, s_req, a.total_k, p.k0, p.lk);
+  p.prefix = a.prefix ? a.prefix[s_req] : 0;
+  p.t0 = s_tile * span;
+  // keys that the tile's last query sees, the most; and its first, the fewest
+  const int most = visible(min(p.lq, p.t0 + span) - 1, p.lq, p.lk, p.prefix);
+  const int fewest = visible(p.t0, p.lq, p.lk, p.prefix);
+  const int n = (most + kKeys - 1) / kKeys;
+
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&s_tmem)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  // position of a tile's K or V in the order of the loads, in units of SPT slots: the order in
+  // which the MMAs take them
+  auto k_unit = [&](int j) { return NQ == 2 ? 2 * j : (j == 0 ? 0 : 2 * j - 1); };
+  auto v_unit = [&](int j) { return NQ == 2 ? 2 * j + 1 : min(2 * j + 2, n + j); };
+
+  // A row whose sum meets an infinity or a NaN may owe it to a value that it does not see (weight
+  // zero times infinity): then the CTA does its tile once more, with such values taken out of the
+  // V tiles that some of its rows see in part.
+  if (warp < 2) {
+   for (int pass = 0; pass < 2; ++pass) {
+    const int load0 = pass * 2 * n * SPT, job0 = pass * NQ * n;
+    if (warp == 0) {
+      if (lane == 0 && n > 0) {
+        // ---- producer ----
+        bool ok = true;
+        int load = load0;
+        if (pass == 0) {
+          // bytes of whole boxes: what lies out of bounds arrives as zeros
+          mbar_expect_tx(&q_full, (uint32_t)(NQ * HD / 64 * tok * group * 128));
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int kb = 0; kb < HD / 64; ++kb)
+              tma_load_3d(sQ + q * C::Q_TILE + kb * 16384, &tmQ, &q_full, kb * 64, kv * group,
+                          p.q0 + p.t0 + q * tok);
+        }
+        auto slot_of = [&]() -> uint8_t* {
+          const int s = load % SLOTS;
+          if (load >= SLOTS)
+            ok = ok && mbar_wait(&empty[s], (load / SLOTS - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
+          if (!ok) return nullptr;
+          mbar_expect_tx(&full[s], C::SLOT);
+          ++load;
+          return base + s * C::SLOT;
+        };
+        auto load_k = [&](int j) {
+#pragma unroll
+          for (int h = 0; h < SPT; ++h) {
+            uint8_t* dst = slot_of();
+            if (!dst) return;
+            uint64_t* bar = &full[(load - 1) % SLOTS];
+#pragma unroll
+            for (int kb = 0; kb < HD / 64 / SPT; ++kb)
+              tma_load_3d(dst + kb * 16384, &tmK, bar, (h * (HD / 64 / SPT) + kb) * 64, kv,
+                          p.k0 + j * kKeys);
+          }
+        };
+        auto load_v = [&](int j) {
+#pragma unroll
+          for (int h = 0; h < SPT; ++h) {
+            uint8_t* dst = slot_of();
+            if (!dst) return;
+            uint64_t* bar = &full[(load - 1) % SLOTS];
+#pragma unroll
+            for (int kb = 0; kb < HD / 64; ++kb)
+              tma_load_3d(dst + kb * (C::VKEYS * 128), &tmV, bar, kb * 64, kv,
+                          p.k0 + j * kKeys + h * C::VKEYS);
+          }
+        };
+        if constexpr (NQ == 2) {
+          for (int j = 0; j < n && ok; ++j) {
+            load_k(j);
+            if (ok) load_v(j);
+          }
+        } else {
+          load_k(0);
+          for (int j = 0; j < n && ok; ++j) {
+            if (j + 1 < n) load_k(j + 1);
+            if (ok) load_v(j);
+          }
+        }
+        // no copy into this CTA's shared memory may be in flight when it exits
+        mbar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
+        for (int l = max(load0, load - SLOTS); l < load; ++l)
+          mbar_wait(&full[l % SLOTS], (l / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (lane == 0 && n > 0) {
+        // ---- MMA issuer: QK 0, QK 1, then P·V i and QK i + 2 in turn ----
+        constexpr uint32_t id_s = tc::idesc_f16<T>(128, kKeys);
+        constexpr uint32_t id_o = tc::idesc_f16<T>(128, HD) | (1u << 16);  // V is MN-major
+        const uint32_t ring = smem_u32(base);
+        const int jobs = NQ * n;
+        bool ok = mbar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_MMA);
+        auto full_of = [&](int load) {
+          return mbar_wait(&full[load % SLOTS], (load / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
+        };
+        auto qk = [&](int i) {
+          const int q = NQ == 2 ? i & 1 : 0, j = NQ == 2 ? i >> 1 : i, buf = (job0 + i) & 1;
+          const int load = load0 + k_unit(j) * SPT;
+#pragma unroll
+          for (int h = 0; h < SPT; ++h) {
+            if (!ok || !(ok = full_of(load + h))) return;
+            tc_fence_after();
+            const uint32_t sb = ring + ((load + h) % SLOTS) * C::SLOT;
+#pragma unroll
+            for (int kb = 0; kb < HD / 64 / SPT; ++kb) {
+              const int qb = h * (HD / 64 / SPT) + kb;
+              const uint64_t da = tc::desc_sw128(smem_u32(sQ + q * C::Q_TILE + qb * 16384));
+              const uint64_t db = tc::desc_sw128(sb + kb * 16384);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc::umma_f16(tmem + buf * kKeys, da + 2 * k, db + 2 * k, id_s, (qb | k) != 0);
+            }
+            if (q == NQ - 1) umma_commit(&empty[(load + h) % SLOTS]);
+          }
+          umma_commit(&s_full[buf]);
+        };
+        auto pv = [&](int i) {
+          const int q = NQ == 2 ? i & 1 : 0, j = NQ == 2 ? i >> 1 : i, buf = (job0 + i) & 1;
+          const int load = load0 + v_unit(j) * SPT;
+          if (!ok || !(ok = mbar_wait(&p_full[buf], ((job0 + i) >> 1) & 1, a.err,
+                                      tc::ERR_TIMEOUT_MMA)))
+            return;
+#pragma unroll
+          for (int h = 0; h < SPT; ++h) {
+            if (!(ok = full_of(load + h))) return;
+            tc_fence_after();
+            const uint32_t sv = ring + ((load + h) % SLOTS) * C::SLOT;
+#pragma unroll
+            for (int k = 0; k < C::VKEYS / 16; ++k)  // 16 keys (2048 bytes of V rows) a step
+              umma_f16_ta(tmem + C::O_COL + q * HD, tmem + buf * kKeys + (h * C::VKEYS / 16 + k) * 8,
+                          sdesc<128>(sv + k * 2048, 1024, C::VKEYS * 128), id_o, (j | h | k) != 0);
+            if (q == NQ - 1) umma_commit(&empty[(load + h) % SLOTS]);
+          }
+          umma_commit(&pv_done[buf]);
+        };
+        qk(0);
+        if (jobs > 1) qk(1);
+        for (int i = 0; i < jobs && ok; ++i) {
+          pv(i);
+          if (i + 2 < jobs) qk(i + 2);
+        }
+        // every issued MMA completes before TMEM is released
+        umma_commit(&drain);
+        mbar_wait(&drain, pass, a.err, tc::ERR_TIMEOUT_MMA, false);
+      }
+      __syncwarp();
+    }
+    if (!block_any<C::THREADS>(false)) break;
+   }
+  } else {
+   for (int pass = 0; pass < 2; ++pass) {
+      bool again = false;
+      const int load0 = pass * 2 * n * SPT, job0 = pass * NQ * n;
+      // ---- softmax and output: one thread per query row ----
+      const int wg = (warp - 2) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
+      const uint32_t tl = tmem + ((uint32_t)(q4 * 32) << 16);
+      const uint32_t tO = tl + C::O_COL + wg * HD;
+      const int i = p.t0 + wg * tok + r / group;     // the row's query
+      const bool row = r < tok * group && i < p.lq;
+      const int mine = row ? visible(i, p.lq, p.lk, p.prefix) : 0;
+      // keys below this need no mask in this warpgroup's rows
+      const int clear = p.t0 + wg * tok < p.lq ? visible(p.t0 + wg * tok, p.lq, p.lk, p.prefix) : 0;
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        const int job = job0 + (NQ == 2 ? 2 * j + wg : j), buf = job & 1;
+        if (ok) ok = mbar_wait(&s_full[buf], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        ok = __all_sync(~0u, ok);
+        if (ok) {
+          tc_fence_after();
+          // The logits are read twice, 32 at a time: for the maximum, then for the weights. Kept in
+          // registers in between they would not leave room for anything else.
+          const uint32_t tS = tl + buf * kKeys;
+          const bool part = (j + 1) * kKeys > clear;
+          const int lim = mine - j * kKeys;
+          const bool flip = a.c <= 0.f;  // the largest logit is not the largest product: scale first
+          const float c = flip ? 1.f : a.c;
+          auto logits = [&](int q, float (&s)[32]) {
+            if (flip)
+#pragma unroll
+              for (int u = 0; u < 32; ++u) s[u] *= a.c;
+            if (part)
+#pragma unroll
+              for (int u = 0; u < 32; ++u) s[u] = 32 * q + u < lim ? s[u] : -INFINITY;
+          };
+          float s[2][32];
+          float top = -INFINITY;
+          tmem_ld32_async(tS, reinterpret_cast<uint32_t*>(s[0]));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            tmem_wait_ld();
+            // the chunk after this one (behind the last: the first again, for the weights)
+            tmem_ld32_async(tS + 32 * ((q + 1) % 4), reinterpret_cast<uint32_t*>(s[(q + 1) & 1]));
+            logits(q, s[q & 1]);
+            top = fmaxf(top, max32(s[q & 1]));
+          }
+          top *= c;
+          if (j == 0) {
+            m = top;
+          } else if (__any_sync(~0u, top > m + kPromptGrow)) {
+            // the sums so far are complete once the P·V before has finished
+            const int prev = NQ == 2 ? job - 2 : job - 1;
+            ok = mbar_wait(&pv_done[prev & 1], (prev >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+            ok = __all_sync(~0u, ok);
+            if (ok) {
+              float al = 1.f;
+              if (top > m + kPromptGrow) {
+                al = m == -INFINITY ? 0.f : exp2_fast(m - top);
+                m = top;
+                l *= al;
+              }
+              tc_fence_after();
+#pragma unroll 1
+              for (int d = 0; d < HD; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(tO + d, o);
+#pragma unroll
+                for (int u = 0; u < 32; ++u)
+                  o[u] = __float_as_uint(__uint_as_float(o[u]) * al);
+                tmem_st32(tO + d, o);
+              }
+            }
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            tmem_wait_ld();
+            if (q < 3)
+              tmem_ld32_async(tS + 32 * (q + 1), reinterpret_cast<uint32_t*>(s[(q + 1) & 1]));
+            logits(q, s[q & 1]);
+            uint32_t w[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+              const float e0 = exp2_fast(fmaf(s[q & 1][2 * u], c, -ref));
+              const float e1 = exp2_fast(fmaf(s[q & 1][2 * u + 1], c, -ref));
+              s0 += e0;
+              s1 += e1;
+              // weights in the type of V, as a 16-bit product asks; their sum is of the fp32 ones
+              w[u] = Tr<T>::pack(e0, e1);
+            }
+            // over logits that have been read: chunk q ends at column 16(q + 1)
+            tmem_st16(tS + 16 * q, w);
+          }
+          l += s0 + s1;
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        if (pass == 1 && (j + 1) * kKeys > fewest) {
+          // V rows of this tile, in halves for two warpgroups: values that are no numbers become
+          // zero; s_bad keeps the first key of the request that lost one
+          const int load = load0 + v_unit(j) * SPT;
+#pragma unroll
+          for (int h = 0; h < SPT; ++h) {
+            const int s = (load + h) % SLOTS;
+            if (ok) ok = mbar_wait(&full[s], ((load + h) / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+            ok = __all_sync(~0u, ok);
+            if (!ok) break;
+            for (int v = tid - 64; v < C::SLOT / 16; v += NQ * 128) {
+              const int key = j * kKeys + h * C::VKEYS + (v / 8) % C::VKEYS;
+              uint4* at = reinterpret_cast<uint4*>(base + s * C::SLOT) + v;
+              uint4 x = *at;
+              T* e = reinterpret_cast<T*>(&x);
+              bool hit = false;
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                if (!isfinite(Tr<T>::f(e[u]))) {
+                  e[u] = Tr<T>::t(0.f);
+                  hit = true;
+                }
+              if (hit) {
+                *at = x;
+                if (key < p.lk) atomicMin(&s_bad, key);
+              }
+            }
+          }
+          fence_async_smem();
+          named_sync<1, NQ * 128>();
+        }
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&p_full[buf]);
+      }
+      if (n > 0) {
+        const int last = job0 + (NQ == 2 ? 2 * (n - 1) + wg : n - 1);
+        if (ok) ok = mbar_wait(&pv_done[last & 1], (last >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        ok = __all_sync(~0u, ok);
+        tc_fence_after();
+      }
+      // ---- o = O / l ----
+      T* out = reinterpret_cast<T*>(a.out) + (int64_t)(p.q0 + i) * a.o_tok +
+               (int64_t)(kv * group + r % group) * a.o_head;
+      const float inv = 1.f / l;
+      bool odd = false, all = true;  // some, and every, element that is no number
+#pragma unroll 1
+      for (int d = 0; d < HD; d += 32) {
+        uint32_t o[32];
+        if (n > 0 && ok) tmem_ld32(tO + d, o);
+        uint4 pk[4];
+        uint32_t* pw = reinterpret_cast<uint32_t*>(pk);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          float x = __uint_as_float(o[2 * u]) * inv, y = __uint_as_float(o[2 * u + 1]) * inv;
+          if (mine == 0) x = y = 0.f;
+          else if (!ok) x = y = NAN;
+          const bool fx = isfinite(x), fy = isfinite(y);
+          odd |= !fx || !fy;
+          all &= !fx && !fy;
+          pw[u] = Tr<T>::pack(x, y);
+        }
+        if (row)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) reinterpret_cast<uint4*>(out + d)[u] = pk[u];
+      }
+      tc_fence_before();
+      again = row && odd && ok;
+      if (pass == 1) {
+        named_sync<1, NQ * 128>();  // s_bad is final, and so is the other warpgroup's tile
+        // rows that do see a value that was taken out, unless they are NaN throughout as it is
+        unsigned redo = __ballot_sync(~0u, row && ok && mine > s_bad && !all);
+        while (redo) {
+          const int src = __ffs(redo) - 1;
+          redo &= redo - 1;
+          const int rr = q4 * 32 + src, ii = p.t0 + wg * tok + rr / group;
+          const int64_t h = kv * group + rr % group;
+          const PromptKV<T> src_kv{
+              reinterpret_cast<const T*>(a.k) + p.k0 * a.k_tok + kv * a.k_head,
+              reinterpret_cast<const T*>(a.v) + p.k0 * a.v_tok + kv * a.v_head, a.k_tok, a.v_tok};
+          attend_row(reinterpret_cast<const T*>(a.q) + (p.q0 + ii) * a.q_tok + h * a.q_head, HD,
+                     visible(ii, p.lq, p.lk, p.prefix), a.c, src_kv,
+                     reinterpret_cast<T*>(a.out) + (p.q0 + ii) * a.o_tok + h * a.o_head);
+        }
+      }
+      if (!block_any<C::THREADS>(again)) break;
+   }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
 }
 
 }  // namespace paged
