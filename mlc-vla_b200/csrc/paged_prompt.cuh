@@ -90,7 +90,10 @@ struct PromptCfg {
   static constexpr int SLOTS = HD == 64 ? 8 : 5;
   static constexpr int Q_TILE = 128 * HD * 2;
   static constexpr int SMEM = NQ * Q_TILE + SLOTS * SLOT + 1024;
-  static constexpr int THREADS = 64 + NQ * 128;    // producer, MMA; softmax
+  static constexpr int THREADS = 128 + NQ * 128;   // producer, MMA (and two idle warps); softmax
+  // of every four pairs of exponentials, those on the FMA pipe: with two tiles of rows the special-
+  // function units need as long as the tensor cores
+  static constexpr int POLY = NQ == 2 ? 1 : 0;
   static constexpr int VKEYS = kKeys / SPT;         // keys of a V slot
   // tensor memory: two tiles of logits, each overlaid by its weights, then the sums
   static constexpr int O_COL = 256;
@@ -100,17 +103,17 @@ struct PromptTile {
   int q0, lq, k0, lk, prefix, t0;
 };
 
-// largest of 32 logits, in four chains
-__device__ __forceinline__ float max32(const float (&s)[32]) {
+// largest of 128 logits, in four chains
+__device__ __forceinline__ float max128(const float (&s)[128]) {
   float a = s[0], b = s[1], c = s[2], d = s[3];
 #pragma unroll
-  for (int j = 4; j < 32; j += 4) {
-    a = fmaxf(a, s[j]);
-    b = fmaxf(b, s[j + 1]);
-    c = fmaxf(c, s[j + 2]);
-    d = fmaxf(d, s[j + 3]);
+  for (int j = 4; j < 124; j += 8) {
+    a = max3(a, s[j], s[j + 1]);
+    b = max3(b, s[j + 2], s[j + 3]);
+    c = max3(c, s[j + 4], s[j + 5]);
+    d = max3(d, s[j + 6], s[j + 7]);
   }
-  return fmaxf(fmaxf(a, b), fmaxf(c, d));
+  return fmaxf(max3(a, s[124], s[125]), fmaxf(max3(b, s[126], s[127]), fmaxf(c, d)));
 }
 
 template <typename T, int HD>
@@ -231,7 +234,12 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
   // A row whose sum meets an infinity or a NaN may owe it to a value that it does not see (weight
   // zero times infinity): then the CTA does its tile once more, with such values taken out of the
   // V tiles that some of its rows see in part.
-  if (warp < 2) {
+  //
+  // A row of 128 logits takes more registers than 1/12 of an SM's: where there are twelve warps, the
+  // first warpgroup gives some of its own. (80 + 2·208)·128 of the 168·384 that the block was
+  // launched with.
+  if (warp < 4) {
+   if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
    for (int pass = 0; pass < 2; ++pass) {
     const int load0 = pass * 2 * n * SPT, job0 = pass * NQ * n;
     if (warp == 0) {
@@ -252,7 +260,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         auto slot_of = [&]() -> uint8_t* {
           const int s = load % SLOTS;
           if (load >= SLOTS)
-            ok = ok && mbar_wait(&empty[s], (load / SLOTS - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
+            ok = ok && bar_wait(&empty[s], (load / SLOTS - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
           if (!ok) return nullptr;
           mbar_expect_tx(&full[s], C::SLOT);
           ++load;
@@ -295,9 +303,9 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           }
         }
         // no copy into this CTA's shared memory may be in flight when it exits
-        mbar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
+        bar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
         for (int l = max(load0, load - SLOTS); l < load; ++l)
-          mbar_wait(&full[l % SLOTS], (l / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
+          bar_wait(&full[l % SLOTS], (l / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
       }
       __syncwarp();
     } else if (warp == 1) {
@@ -307,9 +315,9 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         constexpr uint32_t id_o = tc::idesc_f16<T>(128, HD) | (1u << 16);  // V is MN-major
         const uint32_t ring = smem_u32(base);
         const int jobs = NQ * n;
-        bool ok = mbar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_MMA);
+        bool ok = bar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_MMA);
         auto full_of = [&](int load) {
-          return mbar_wait(&full[load % SLOTS], (load / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
+          return bar_wait(&full[load % SLOTS], (load / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
         };
         auto qk = [&](int i) {
           const int q = NQ == 2 ? i & 1 : 0, j = NQ == 2 ? i >> 1 : i, buf = (job0 + i) & 1;
@@ -335,7 +343,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         auto pv = [&](int i) {
           const int q = NQ == 2 ? i & 1 : 0, j = NQ == 2 ? i >> 1 : i, buf = (job0 + i) & 1;
           const int load = load0 + v_unit(j) * SPT;
-          if (!ok || !(ok = mbar_wait(&p_full[buf], ((job0 + i) >> 1) & 1, a.err,
+          if (!ok || !(ok = bar_wait(&p_full[buf], ((job0 + i) >> 1) & 1, a.err,
                                       tc::ERR_TIMEOUT_MMA)))
             return;
 #pragma unroll
@@ -359,18 +367,19 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         }
         // every issued MMA completes before TMEM is released
         umma_commit(&drain);
-        mbar_wait(&drain, pass, a.err, tc::ERR_TIMEOUT_MMA, false);
+        bar_wait(&drain, pass, a.err, tc::ERR_TIMEOUT_MMA, false);
       }
       __syncwarp();
     }
     if (!block_any<C::THREADS>(false)) break;
    }
   } else {
+   if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
    for (int pass = 0; pass < 2; ++pass) {
       bool again = false;
       const int load0 = pass * 2 * n * SPT, job0 = pass * NQ * n;
       // ---- softmax and output: one thread per query row ----
-      const int wg = (warp - 2) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
+      const int wg = (warp - 4) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
       const uint32_t tl = tmem + ((uint32_t)(q4 * 32) << 16);
       const uint32_t tO = tl + C::O_COL + wg * HD;
       const int i = p.t0 + wg * tok + r / group;     // the row's query
@@ -382,43 +391,33 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       bool ok = true;
       for (int j = 0; j < n; ++j) {
         const int job = job0 + (NQ == 2 ? 2 * j + wg : j), buf = job & 1;
-        if (ok) ok = mbar_wait(&s_full[buf], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        if (ok) ok = bar_wait(&s_full[buf], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
         ok = __all_sync(~0u, ok);
         if (ok) {
           tc_fence_after();
-          // The logits are read twice, 32 at a time: for the maximum, then for the weights. Kept in
-          // registers in between they would not leave room for anything else.
-          const uint32_t tS = tl + buf * kKeys;
-          const bool part = (j + 1) * kKeys > clear;
-          const int lim = mine - j * kKeys;
-          const bool flip = a.c <= 0.f;  // the largest logit is not the largest product: scale first
-          const float c = flip ? 1.f : a.c;
-          auto logits = [&](int q, float (&s)[32]) {
-            if (flip)
+          float s[128];
 #pragma unroll
-              for (int u = 0; u < 32; ++u) s[u] *= a.c;
-            if (part)
+          for (int q = 0; q < 4; ++q)
+            tmem_ld32_async(tl + buf * kKeys + 32 * q, reinterpret_cast<uint32_t*>(s) + 32 * q);
+          tmem_wait_ld();
+          float c = a.c;
+          if (c <= 0.f) {  // the largest logit is not the largest product: scale first
 #pragma unroll
-              for (int u = 0; u < 32; ++u) s[u] = 32 * q + u < lim ? s[u] : -INFINITY;
-          };
-          float s[2][32];
-          float top = -INFINITY;
-          tmem_ld32_async(tS, reinterpret_cast<uint32_t*>(s[0]));
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            tmem_wait_ld();
-            // the chunk after this one (behind the last: the first again, for the weights)
-            tmem_ld32_async(tS + 32 * ((q + 1) % 4), reinterpret_cast<uint32_t*>(s[(q + 1) & 1]));
-            logits(q, s[q & 1]);
-            top = fmaxf(top, max32(s[q & 1]));
+            for (int u = 0; u < 128; ++u) s[u] *= c;
+            c = 1.f;
           }
-          top *= c;
+          if ((j + 1) * kKeys > clear) {
+            const int lim = mine - j * kKeys;
+#pragma unroll
+            for (int u = 0; u < 128; ++u) s[u] = u < lim ? s[u] : -INFINITY;
+          }
+          const float top = max128(s) * c;
           if (j == 0) {
             m = top;
           } else if (__any_sync(~0u, top > m + kPromptGrow)) {
             // the sums so far are complete once the P·V before has finished
             const int prev = NQ == 2 ? job - 2 : job - 1;
-            ok = mbar_wait(&pv_done[prev & 1], (prev >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+            ok = bar_wait(&pv_done[prev & 1], (prev >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
             ok = __all_sync(~0u, ok);
             if (ok) {
               float al = 1.f;
@@ -440,27 +439,31 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             }
           }
           const float ref = m == -INFINITY ? 0.f : m;
-          float s0 = 0.f, s1 = 0.f;
+          const uint64_t c2 = pack2(c, c), r2 = pack2(-ref, -ref);
+          uint64_t sum0 = 0, sum1 = 0;  // two zeros each
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            tmem_wait_ld();
-            if (q < 3)
-              tmem_ld32_async(tS + 32 * (q + 1), reinterpret_cast<uint32_t*>(s[(q + 1) & 1]));
-            logits(q, s[q & 1]);
             uint32_t w[16];
 #pragma unroll
             for (int u = 0; u < 16; ++u) {
-              const float e0 = exp2_fast(fmaf(s[q & 1][2 * u], c, -ref));
-              const float e1 = exp2_fast(fmaf(s[q & 1][2 * u + 1], c, -ref));
-              s0 += e0;
-              s1 += e1;
+              const int at = 32 * q + 2 * u;
+              uint64_t x = fma2(pack2(s[at], s[at + 1]), c2, r2);
+              if (u % 4 < C::POLY) {
+                x = exp2_poly(x);
+              } else {
+                const float2 f = unpack2(x);
+                x = pack2(exp2_fast(f.x), exp2_fast(f.y));
+              }
+              if (u & 1) sum1 = add2(sum1, x);
+              else sum0 = add2(sum0, x);
               // weights in the type of V, as a 16-bit product asks; their sum is of the fp32 ones
-              w[u] = Tr<T>::pack(e0, e1);
+              const float2 e = unpack2(x);
+              w[u] = Tr<T>::pack(e.x, e.y);
             }
-            // over logits that have been read: chunk q ends at column 16(q + 1)
-            tmem_st16(tS + 16 * q, w);
+            tmem_st16(tl + buf * kKeys + 16 * q, w);
           }
-          l += s0 + s1;
+          const float2 sums = unpack2(add2(sum0, sum1));
+          l += sums.x + sums.y;
           tmem_wait_st();
           tc_fence_before();
         }
@@ -471,10 +474,10 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
 #pragma unroll
           for (int h = 0; h < SPT; ++h) {
             const int s = (load + h) % SLOTS;
-            if (ok) ok = mbar_wait(&full[s], ((load + h) / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+            if (ok) ok = bar_wait(&full[s], ((load + h) / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_EPI);
             ok = __all_sync(~0u, ok);
             if (!ok) break;
-            for (int v = tid - 64; v < C::SLOT / 16; v += NQ * 128) {
+            for (int v = tid - 128; v < C::SLOT / 16; v += NQ * 128) {
               const int key = j * kKeys + h * C::VKEYS + (v / 8) % C::VKEYS;
               uint4* at = reinterpret_cast<uint4*>(base + s * C::SLOT) + v;
               uint4 x = *at;
@@ -500,7 +503,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       }
       if (n > 0) {
         const int last = job0 + (NQ == 2 ? 2 * (n - 1) + wg : n - 1);
-        if (ok) ok = mbar_wait(&pv_done[last & 1], (last >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        if (ok) ok = bar_wait(&pv_done[last & 1], (last >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
         ok = __all_sync(~0u, ok);
         tc_fence_after();
       }

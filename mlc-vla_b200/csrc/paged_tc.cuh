@@ -121,6 +121,77 @@ __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// tc::mbar_wait without its call, for kernels that shift registers between warps (setmaxnreg allows
+// no call)
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* err, int code,
+                                         bool bail = true) {
+  if (tc::mbar_try(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer();
+  for (uint32_t it = 1;; ++it) {
+    if (tc::mbar_try(bar, parity)) return true;
+    if ((it & 127) == 0) {
+      if (globaltimer() - t0 > tc::kTimeoutNs) {
+        atomicCAS(err, 0, code);
+        return false;
+      }
+      if (bail && (it & 8191) == 0 && *(volatile int*)err != 0) return false;
+    }
+  }
+}
+
+// ---- two fp32 at a time: the packed forms issue once for both ----
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x for two values x ≤ 127 on the FMA pipe, for kernels that the 16 exponentials a clock of the
+// special-function units hold up: n = x rounded to a whole number (the last bits of x + 1.5·2^23),
+// 2^(x−n) by a polynomial of degree 4 on [−1/2, 1/2] (minimax of the relative error, 2.6e-6, found
+// by an exchange of its extrema), times 2^n from the exponent field. Below −127 the field is 0 and
+// so is the result, also for −∞; NaN stays NaN.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t v) {
+  float2 x = unpack2(v);
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // −127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  v = pack2(x.x, x.y);
+  const uint64_t t = add2(v, pack2(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), v);
+  uint64_t p = fma2(f, pack2(0.009570102207f, 0.009570102207f), pack2(0.05591785908f, 0.05591785908f));
+  p = fma2(f, p, pack2(0.24024744332f, 0.24024744332f));
+  p = fma2(f, p, pack2(0.69312179089f, 0.69312179089f));
+  p = fma2(f, p, pack2(0.99999928474f, 0.99999928474f));
+  const float2 n = unpack2(t);
+  return mul2(p, pack2(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u),
+                       __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u)));
+}
+
 // largest of a warp's values (NaN counts as smaller), one instruction
 __device__ __forceinline__ float warp_max_f32(float v) {
   float r;
