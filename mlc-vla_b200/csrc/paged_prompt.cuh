@@ -309,11 +309,12 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       }
       __syncwarp();
     } else if (warp == 1) {
-      if (lane == 0 && n > 0) {
+      if (n > 0) {
         // ---- MMA issuer: QK 0, QK 1, then P·V i and QK i + 2 in turn ----
         constexpr uint32_t id_s = tc::idesc_f16<T>(128, kKeys);
         constexpr uint32_t id_o = tc::idesc_f16<T>(128, HD) | (1u << 16);  // V is MN-major
-        const uint32_t ring = smem_u32(base);
+        const uint32_t ring = __shfl_sync(~0u, smem_u32(base), 0), tm = __shfl_sync(~0u, tmem, 0);
+        const uint32_t qs = ring + SLOTS * C::SLOT;
         const int jobs = NQ * n;
         bool ok = bar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_MMA);
         auto full_of = [&](int load) {
@@ -326,38 +327,45 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           for (int h = 0; h < SPT; ++h) {
             if (!ok || !(ok = full_of(load + h))) return;
             tc_fence_after();
-            const uint32_t sb = ring + ((load + h) % SLOTS) * C::SLOT;
+            const int slot = (load + h) % SLOTS;
+            const uint64_t da = tc::desc_sw128(qs + q * C::Q_TILE + h * (HD / 64 / SPT) * 16384);
+            const uint64_t db = tc::desc_sw128(ring + slot * C::SLOT);
+            if (elect_one()) {
 #pragma unroll
-            for (int kb = 0; kb < HD / 64 / SPT; ++kb) {
-              const int qb = h * (HD / 64 / SPT) + kb;
-              const uint64_t da = tc::desc_sw128(smem_u32(sQ + q * C::Q_TILE + qb * 16384));
-              const uint64_t db = tc::desc_sw128(sb + kb * 16384);
+              for (int kb = 0; kb < HD / 64 / SPT; ++kb)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                tc::umma_f16(tmem + buf * kKeys, da + 2 * k, db + 2 * k, id_s, (qb | k) != 0);
+                for (int k = 0; k < 4; ++k)
+                  tc::umma_f16(tm + buf * kKeys, da + 1024 * kb + 2 * k, db + 1024 * kb + 2 * k, id_s,
+                               (h | kb | k) != 0);
+              if (q == NQ - 1) umma_commit(&empty[slot]);
+              if (h == SPT - 1) umma_commit(&s_full[buf]);
             }
-            if (q == NQ - 1) umma_commit(&empty[(load + h) % SLOTS]);
+            __syncwarp();
           }
-          umma_commit(&s_full[buf]);
         };
         auto pv = [&](int i) {
           const int q = NQ == 2 ? i & 1 : 0, j = NQ == 2 ? i >> 1 : i, buf = (job0 + i) & 1;
           const int load = load0 + v_unit(j) * SPT;
           if (!ok || !(ok = bar_wait(&p_full[buf], ((job0 + i) >> 1) & 1, a.err,
-                                      tc::ERR_TIMEOUT_MMA)))
+                                     tc::ERR_TIMEOUT_MMA)))
             return;
 #pragma unroll
           for (int h = 0; h < SPT; ++h) {
             if (!(ok = full_of(load + h))) return;
             tc_fence_after();
-            const uint32_t sv = ring + ((load + h) % SLOTS) * C::SLOT;
+            const int slot = (load + h) % SLOTS;
+            const uint64_t dv = sdesc<128>(ring + slot * C::SLOT, 1024, C::VKEYS * 128);
+            const uint32_t tp = tm + buf * kKeys + h * (C::VKEYS / 2), to = tm + C::O_COL + q * HD;
+            const uint32_t more = (j | h) != 0;
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < C::VKEYS / 16; ++k)  // 16 keys (2048 bytes of V rows) a step
-              umma_f16_ta(tmem + C::O_COL + q * HD, tmem + buf * kKeys + (h * C::VKEYS / 16 + k) * 8,
-                          sdesc<128>(sv + k * 2048, 1024, C::VKEYS * 128), id_o, (j | h | k) != 0);
-            if (q == NQ - 1) umma_commit(&empty[(load + h) % SLOTS]);
+              for (int k = 0; k < C::VKEYS / 16; ++k)  // 16 keys (2048 bytes of V rows) a step
+                umma_f16_ta(to, tp + 8 * k, dv + 128 * k, id_o, k == 0 ? more : 1u);
+              if (q == NQ - 1) umma_commit(&empty[slot]);
+              if (h == SPT - 1) umma_commit(&pv_done[buf]);
+            }
+            __syncwarp();
           }
-          umma_commit(&pv_done[buf]);
         };
         qk(0);
         if (jobs > 1) qk(1);
@@ -366,7 +374,8 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           if (i + 2 < jobs) qk(i + 2);
         }
         // every issued MMA completes before TMEM is released
-        umma_commit(&drain);
+        if (elect_one()) umma_commit(&drain);
+        __syncwarp();
         bar_wait(&drain, pass, a.err, tc::ERR_TIMEOUT_MMA, false);
       }
       __syncwarp();

@@ -139,6 +139,17 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* er
   }
 }
 
+// One thread of a converged warp. Tensor-core instructions are issued by a whole warp's control flow
+// under this predicate: their operands then stay in uniform registers. From a branch on the lane
+// number each of them took over 100 clocks to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(r));
+  return r != 0;
+}
+
 // ---- two fp32 at a time: the packed forms issue once for both ----
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
   uint64_t r;
