@@ -91,9 +91,6 @@ struct PromptCfg {
   static constexpr int Q_TILE = 128 * HD * 2;
   static constexpr int SMEM = NQ * Q_TILE + SLOTS * SLOT + 1024;
   static constexpr int THREADS = 128 + NQ * 128;   // producer, MMA (and two idle warps); softmax
-  // of every four pairs of exponentials, those on the FMA pipe: with two tiles of rows the special-
-  // function units need as long as the tensor cores
-  static constexpr int POLY = NQ == 2 ? 1 : 0;
   static constexpr int VKEYS = kKeys / SPT;         // keys of a V slot
   // tensor memory: two tiles of logits, each overlaid by its weights, then the sums
   static constexpr int O_COL = 256;
@@ -127,8 +124,8 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = base + SLOTS * C::SLOT;
-  __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, s_full[2], p_full[2],
-      pv_done[2], drain;
+  __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, s_full[2],
+      p_full[2][2], pv_done[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ int s_scan[C::THREADS / 32], s_req, s_tile, s_bad;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -143,7 +140,8 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
     mbar_init(&q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i][0], 4);
+      mbar_init(&p_full[i][1], 4);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(&drain, 1);
@@ -346,23 +344,26 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         auto pv = [&](int i) {
           const int q = NQ == 2 ? i & 1 : 0, j = NQ == 2 ? i >> 1 : i, buf = (job0 + i) & 1;
           const int load = load0 + v_unit(j) * SPT;
-          if (!ok || !(ok = bar_wait(&p_full[buf], ((job0 + i) >> 1) & 1, a.err,
-                                     tc::ERR_TIMEOUT_MMA)))
-            return;
+          // V is there before the weights are; these come in two halves of the keys
 #pragma unroll
-          for (int h = 0; h < SPT; ++h) {
-            if (!(ok = full_of(load + h))) return;
+          for (int h = 0; h < SPT; ++h)
+            if (!ok || !(ok = full_of(load + h))) return;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!(ok = bar_wait(&p_full[buf][h], ((job0 + i) >> 1) & 1, a.err, tc::ERR_TIMEOUT_MMA)))
+              return;
             tc_fence_after();
-            const int slot = (load + h) % SLOTS;
-            const uint64_t dv = sdesc<128>(ring + slot * C::SLOT, 1024, C::VKEYS * 128);
-            const uint32_t tp = tm + buf * kKeys + h * (C::VKEYS / 2), to = tm + C::O_COL + q * HD;
+            const int slot = (load + h * (SPT - 1)) % SLOTS;
+            const uint64_t dv = sdesc<128>(ring + slot * C::SLOT, 1024, C::VKEYS * 128) +
+                                (SPT == 1 ? 512 * h : 0);
+            const uint32_t tp = tm + buf * kKeys + 32 * h, to = tm + C::O_COL + q * HD;
             const uint32_t more = (j | h) != 0;
             if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < C::VKEYS / 16; ++k)  // 16 keys (2048 bytes of V rows) a step
+              for (int k = 0; k < 4; ++k)  // 16 keys (2048 bytes of V rows) a step
                 umma_f16_ta(to, tp + 8 * k, dv + 128 * k, id_o, k == 0 ? more : 1u);
-              if (q == NQ - 1) umma_commit(&empty[slot]);
-              if (h == SPT - 1) umma_commit(&pv_done[buf]);
+              if (q == NQ - 1 && h >= 2 - SPT) umma_commit(&empty[slot]);
+              if (h == 1) umma_commit(&pv_done[buf]);
             }
             __syncwarp();
           }
@@ -457,12 +458,8 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             for (int u = 0; u < 16; ++u) {
               const int at = 32 * q + 2 * u;
               uint64_t x = fma2(pack2(s[at], s[at + 1]), c2, r2);
-              if (u % 4 < C::POLY) {
-                x = exp2_poly(x);
-              } else {
-                const float2 f = unpack2(x);
-                x = pack2(exp2_fast(f.x), exp2_fast(f.y));
-              }
+              const float2 f = unpack2(x);
+              x = pack2(exp2_fast(f.x), exp2_fast(f.y));
               if (u & 1) sum1 = add2(sum1, x);
               else sum0 = add2(sum0, x);
               // weights in the type of V, as a 16-bit product asks; their sum is of the fp32 ones
@@ -470,6 +467,12 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
               w[u] = Tr<T>::pack(e.x, e.y);
             }
             tmem_st16(tl + buf * kKeys + 16 * q, w);
+            if (q == 1) {  // the first 64 weights may go
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (pass == 0 && lane == 0) mbar_arrive(&p_full[buf][0]);
+            }
           }
           const float2 sums = unpack2(add2(sum0, sum1));
           l += sums.x + sums.y;
@@ -508,7 +511,10 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           named_sync<1, NQ * 128>();
         }
         __syncwarp();
-        if (ok && lane == 0) mbar_arrive(&p_full[buf]);
+        if (ok && lane == 0) {
+          if (pass == 1) mbar_arrive(&p_full[buf][0]);  // only now is V what it should be
+          mbar_arrive(&p_full[buf][1]);
+        }
       }
       if (n > 0) {
         const int last = job0 + (NQ == 2 ? 2 * (n - 1) + wg : n - 1);

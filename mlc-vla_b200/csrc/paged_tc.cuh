@@ -171,36 +171,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-
-// 2^x for two values x ≤ 127 on the FMA pipe, for kernels that the 16 exponentials a clock of the
-// special-function units hold up: n = x rounded to a whole number (the last bits of x + 1.5·2^23),
-// 2^(x−n) by a polynomial of degree 4 on [−1/2, 1/2] (minimax of the relative error, 2.6e-6, found
-// by an exchange of its extrema), times 2^n from the exponent field. Below −127 the field is 0 and
-// so is the result, also for −∞; NaN stays NaN.
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t v) {
-  float2 x = unpack2(v);
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // −127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
-  v = pack2(x.x, x.y);
-  const uint64_t t = add2(v, pack2(12582912.f, 12582912.f));
-  const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), v);
-  uint64_t p = fma2(f, pack2(0.009570102207f, 0.009570102207f), pack2(0.05591785908f, 0.05591785908f));
-  p = fma2(f, p, pack2(0.24024744332f, 0.24024744332f));
-  p = fma2(f, p, pack2(0.69312179089f, 0.69312179089f));
-  p = fma2(f, p, pack2(0.99999928474f, 0.99999928474f));
-  const float2 n = unpack2(t);
-  return mul2(p, pack2(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u),
-                       __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u)));
 }
 
 // largest of a warp's values (NaN counts as smaller), one instruction
