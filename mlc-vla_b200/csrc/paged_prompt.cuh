@@ -90,7 +90,7 @@ struct PromptCfg {
   static constexpr int SLOTS = HD == 64 ? 8 : 5;
   static constexpr int Q_TILE = 128 * HD * 2;
   static constexpr int SMEM = NQ * Q_TILE + SLOTS * SLOT + 1024;
-  static constexpr int THREADS = 128 + NQ * 128;   // producer, MMA (and two idle warps); softmax
+  static constexpr int THREADS = 128 + NQ * 128;   // producer, MMA issuers (and an idle warp); softmax
   static constexpr int VKEYS = kKeys / SPT;         // keys of a V slot
   // tensor memory: two tiles of logits, each overlaid by its weights, then the sums
   static constexpr int O_COL = 256;
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
   if (tid == 0) {
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], NQ);
     }
     mbar_init(&q_full, 1);
     for (int i = 0; i < 2; ++i) {
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       mbar_init(&p_full[i][1], 4);
       mbar_init(&pv_done[i], 1);
     }
-    mbar_init(&drain, 1);
+    mbar_init(&drain, NQ);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -306,27 +306,29 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           bar_wait(&full[l % SLOTS], (l / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
       }
       __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp <= NQ) {
       if (n > 0) {
-        // ---- MMA issuer: QK 0, QK 1, then P·V i and QK i + 2 in turn ----
+        // ---- MMA issuers: with two tiles of rows a warp for each, so that neither waits for the
+        // other's weights. A tile's logits and weights share their columns, and MMAs of one thread
+        // run in order: P·V j, then the logits that overwrite P.
         constexpr uint32_t id_s = tc::idesc_f16<T>(128, kKeys);
         constexpr uint32_t id_o = tc::idesc_f16<T>(128, HD) | (1u << 16);  // V is MN-major
+        const int q = warp - 1;
         const uint32_t ring = __shfl_sync(~0u, smem_u32(base), 0), tm = __shfl_sync(~0u, tmem, 0);
-        const uint32_t qs = ring + SLOTS * C::SLOT;
-        const int jobs = NQ * n;
+        const uint32_t qs = ring + SLOTS * C::SLOT + q * C::Q_TILE, to = tm + C::O_COL + q * HD;
         bool ok = bar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_MMA);
         auto full_of = [&](int load) {
           return bar_wait(&full[load % SLOTS], (load / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
         };
-        auto qk = [&](int i) {
-          const int q = NQ == 2 ? i & 1 : 0, j = NQ == 2 ? i >> 1 : i, buf = (job0 + i) & 1;
-          const int load = load0 + k_unit(j) * SPT;
+        auto job_of = [&](int j) { return job0 + (NQ == 2 ? 2 * j + q : j); };
+        auto qk = [&](int j) {
+          const int buf = job_of(j) & 1, load = load0 + k_unit(j) * SPT;
 #pragma unroll
           for (int h = 0; h < SPT; ++h) {
             if (!ok || !(ok = full_of(load + h))) return;
             tc_fence_after();
             const int slot = (load + h) % SLOTS;
-            const uint64_t da = tc::desc_sw128(qs + q * C::Q_TILE + h * (HD / 64 / SPT) * 16384);
+            const uint64_t da = tc::desc_sw128(qs + h * (HD / 64 / SPT) * 16384);
             const uint64_t db = tc::desc_sw128(ring + slot * C::SLOT);
             if (elect_one()) {
 #pragma unroll
@@ -335,44 +337,45 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                 for (int k = 0; k < 4; ++k)
                   tc::umma_f16(tm + buf * kKeys, da + 1024 * kb + 2 * k, db + 1024 * kb + 2 * k, id_s,
                                (h | kb | k) != 0);
-              if (q == NQ - 1) umma_commit(&empty[slot]);
               if (h == SPT - 1) umma_commit(&s_full[buf]);
+              umma_commit(&empty[slot]);
             }
             __syncwarp();
           }
         };
-        auto pv = [&](int i) {
-          const int q = NQ == 2 ? i & 1 : 0, j = NQ == 2 ? i >> 1 : i, buf = (job0 + i) & 1;
-          const int load = load0 + v_unit(j) * SPT;
+        auto pv = [&](int j) {
+          const int job = job_of(j), buf = job & 1, load = load0 + v_unit(j) * SPT;
           // V is there before the weights are; these come in two halves of the keys
 #pragma unroll
           for (int h = 0; h < SPT; ++h)
             if (!ok || !(ok = full_of(load + h))) return;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (!(ok = bar_wait(&p_full[buf][h], ((job0 + i) >> 1) & 1, a.err, tc::ERR_TIMEOUT_MMA)))
+            if (!(ok = bar_wait(&p_full[buf][h], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_MMA)))
               return;
             tc_fence_after();
             const int slot = (load + h * (SPT - 1)) % SLOTS;
             const uint64_t dv = sdesc<128>(ring + slot * C::SLOT, 1024, C::VKEYS * 128) +
                                 (SPT == 1 ? 512 * h : 0);
-            const uint32_t tp = tm + buf * kKeys + 32 * h, to = tm + C::O_COL + q * HD;
+            const uint32_t tp = tm + buf * kKeys + 32 * h;
             const uint32_t more = (j | h) != 0;
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)  // 16 keys (2048 bytes of V rows) a step
                 umma_f16_ta(to, tp + 8 * k, dv + 128 * k, id_o, k == 0 ? more : 1u);
-              if (q == NQ - 1 && h >= 2 - SPT) umma_commit(&empty[slot]);
               if (h == 1) umma_commit(&pv_done[buf]);
+              if (h >= 2 - SPT) umma_commit(&empty[slot]);
             }
             __syncwarp();
           }
         };
-        qk(0);
-        if (jobs > 1) qk(1);
-        for (int i = 0; i < jobs && ok; ++i) {
-          pv(i);
-          if (i + 2 < jobs) qk(i + 2);
+        constexpr int kAhead = NQ == 2 ? 1 : 2;  // tiles of logits before the first weights
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+          if (j < n) qk(j);
+        for (int j = 0; j < n && ok; ++j) {
+          pv(j);
+          if (j + kAhead < n) qk(j + kAhead);
         }
         // every issued MMA completes before TMEM is released
         if (elect_one()) umma_commit(&drain);
