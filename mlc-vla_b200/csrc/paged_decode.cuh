@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
   const int group = a.heads / a.cache.kv_heads, chunks = (group + NH - 1) / NH;
   const int subs = a.cache.kv_heads * chunks;
   const int ps = a.cache.page_size, ctas = gridDim.x, cta = blockIdx.x;
+  pdl_trigger();  // every CTA of this grid is resident at once: the joining blocks may move in
 
   if (tid == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
@@ -692,7 +693,6 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
   }
   tc_fence_before();
   __syncthreads();
-  pdl_trigger();
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),

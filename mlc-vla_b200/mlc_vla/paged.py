@@ -20,7 +20,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 from typing import Dict, NamedTuple, Optional
 
 import torch
@@ -98,42 +97,56 @@ def check(device="cuda") -> None:
 def _err_ptr(err: Optional[torch.Tensor], device: torch.device) -> int:
     if err is None:
         return _flag(device).data_ptr()
-    _ints(err, "err", device, 1)
+    _ints(err, "err", device, 1, 1)
     return err.data_ptr()
 
 
-def _ints(t: torch.Tensor, name: str, device: torch.device, dim: int) -> None:
-    if t.dtype != torch.int32 or t.device != device or t.dim() != dim or (
-            t.shape[-1] > 1 and t.stride(-1) != 1) or (
-            dim == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise ValueError(f"{name} must be a {dim}-dimensional int32 tensor on {device}, "
-                         f"contiguous along its last dimension and not expanded")
+# The checks below run on every call of a decode step, so they ask a tensor for each of its
+# properties once.
+
+def _ints(t: torch.Tensor, name: str, device: torch.device, dim: int,
+          n: Optional[int] = None) -> None:
+    shape = t.shape
+    if t.dtype is not torch.int32 or t.device != device or len(shape) != dim:
+        raise ValueError(f"{name} must be a {dim}-dimensional int32 tensor on {device}")
+    if n is not None and shape[0] != n:
+        raise ValueError(f"{name} must hold {n} numbers, not {shape[0]}")
+    if not t.is_contiguous():
+        stride = t.stride()
+        if (shape[-1] > 1 and stride[-1] != 1) or (
+                dim == 2 and shape[0] > 1 and stride[0] < shape[1]):
+            raise ValueError(f"{name} must be contiguous along its last dimension and not expanded")
 
 
-def _rows(t: torch.Tensor, name: str, device: torch.device, dtype, shape=None) -> None:
-    """[tokens, heads, head_dim] in 16 bits, read in 16-byte vectors along the last dimension."""
-    if t.dim() != 3 or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be a [tokens, heads, head_dim] {dtype} tensor on {device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
-    if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16
-                      or any(x % 8 or x == 0 for x in _strides(t))):
+def _rows(t: torch.Tensor, name: str, device: torch.device, dtype, shape=None):
+    """[tokens, heads, head_dim] in 16 bits, read in 16-byte vectors along the last dimension:
+    its start, token stride and head stride."""
+    if t.dtype is not dtype or t.device != device:
+        raise ValueError(f"{name} must be a {dtype} tensor on {device}")
+    have = t.shape
+    if len(have) != 3 or (shape is not None and have != shape):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim]"
+                         + (f" = {tuple(shape)}, not {tuple(have)}" if shape is not None else ""))
+    tokens, heads, dim = have
+    tok, head, last = t.stride()
+    # a stride that no second token or head uses is free: take a valid one
+    if tokens < 2:
+        tok = heads * dim
+    if heads < 2:
+        head = dim
+    ptr = t.data_ptr()
+    if (last != 1 or ptr & 15 or tok & 7 or head & 7 or not tok or not head) and t.numel():
         raise ValueError(f"{name} must be contiguous along its last dimension, with token and "
                          f"head strides that are multiples of 8 elements (not expanded) and a "
                          f"16-byte aligned start")
-
-
-def _strides(t: torch.Tensor):
-    """Token and head stride; one that no second token or head uses is free, so a valid one."""
-    dim = t.shape[2]
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim,
-            t.stride(1) if t.shape[1] > 1 else dim)
+    return ptr, tok, head
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
-    if not t.is_cuda or t.dtype not in _DTYPE:
+    code = _DTYPE.get(t.dtype)
+    if code is None or not t.is_cuda:
         raise ValueError(f"{name} must be a float16 or bfloat16 CUDA tensor")
-    return _DTYPE[t.dtype]
+    return code
 
 
 def _head_dim(d: int) -> None:
@@ -142,35 +155,37 @@ def _head_dim(d: int) -> None:
 
 
 def _cache(c: KVCache8, device: torch.device) -> _lib.Pi0Kv8C:
-    if c.k.dim() != 4 or c.k.shape != c.v.shape:
+    k, v, k_scale, v_scale = c
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError("cache codes must be [pages, kv heads, page, head_dim], alike for k and v")
-    pages, heads, page, dim = c.k.shape
+    pages, heads, page, dim = shape
     _head_dim(dim)
-    for t in (c.k, c.v):
-        if t.dtype != torch.float8_e4m3fn or t.device != device or not t.is_contiguous() or (
-                t.data_ptr() % 16):
-            raise ValueError(f"cache codes must be contiguous, 16-byte aligned float8_e4m3fn "
-                             f"tensors on {device}")
-    for t in (c.k_scale, c.v_scale):
-        if t.dtype != torch.float32 or t.device != device or not t.is_contiguous() or (
-                t.shape != c.k.shape[:2]):
-            raise ValueError(f"cache scales must be contiguous float32 [pages, kv heads] tensors "
-                             f"on {device}")
-    return _lib.Pi0Kv8C(c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(),
-                        pages, page, heads, dim)
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if not (k.dtype is v.dtype is torch.float8_e4m3fn and k.device == device and v.device == device
+            and k.is_contiguous() and v.is_contiguous()) or (kp | vp) & 15:
+        raise ValueError(f"cache codes must be contiguous, 16-byte aligned float8_e4m3fn tensors "
+                         f"on {device}")
+    planes = shape[:2]
+    if not (k_scale.dtype is v_scale.dtype is torch.float32 and k_scale.device == device
+            and v_scale.device == device and k_scale.shape == planes and v_scale.shape == planes
+            and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise ValueError(f"cache scales must be contiguous float32 [pages, kv heads] tensors on "
+                         f"{device}")
+    return _lib.Pi0Kv8C(kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), pages, page, heads, dim)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent without CUDA
 
 
 def _call(name: str, device: torch.device, *args) -> None:
-    lib = _lib.load()
-    if torch.cuda.current_device() == device.index:
-        rc = getattr(lib, name)(*args, _stream(device))
+    f = getattr(_lib._lib or _lib.load(), name)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = f(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args, _stream(device))
+        with torch.cuda.device(index):
+            rc = f(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, None, name)
 
@@ -182,6 +197,22 @@ def _workspace_bytes(device: torch.device, heads: int, kv_heads: int, dim: int, 
     if n < 0:
         raise _lib.Pi0Error(_lib.PI0_ERR_CUDA, "pi0_attention_paged_workspace")
     return n
+
+
+_workspaces: Dict[tuple, torch.Tensor] = {}
+
+
+def _workspace(device: torch.device, heads: int, kv_heads: int, dim: int, page: int) -> torch.Tensor:
+    """Room for the partial sums of one call. Calls on one stream follow each other, so a stream's
+    calls share a buffer; a captured graph may be replayed on any stream and has its own."""
+    n = _workspace_bytes(device, heads, kv_heads, dim, page)
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(n, dtype=torch.uint8, device=device)
+    key = (device.index, _raw_stream(device.index))
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < n:
+        ws = _workspaces[key] = torch.empty(n, dtype=torch.uint8, device=device)
+    return ws
 
 
 def build_slots(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
@@ -200,11 +231,10 @@ def build_slots(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
         raise ValueError("block_table must be a CUDA tensor")
     _ints(block_table, "block_table", dev, 2)
     batch, max_pages = block_table.shape
-    for t, name, n in ((kv_lens, "kv_lens", batch), (new_lens, "new_lens", batch),
-                       (free_pos, "free_pos", 1), (free_pages, "free_pages", None)):
-        _ints(t, name, dev, 1)
-        if n is not None and t.shape[0] != n:
-            raise ValueError(f"{name} must hold {n} numbers")
+    _ints(kv_lens, "kv_lens", dev, 1, batch)
+    _ints(new_lens, "new_lens", dev, 1, batch)
+    _ints(free_pos, "free_pos", dev, 1, 1)
+    _ints(free_pages, "free_pages", dev, 1)
     if page_size < 1 or num_tokens < 0 or max_pages < 1:
         raise ValueError("page_size and the block table's columns must be positive, num_tokens "
                          "not negative")
@@ -215,16 +245,17 @@ def build_slots(kv_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     if batch > 16384:
         raise ValueError("at most 16384 requests")
     # one allocation for the five results
-    buf = torch.empty(2 * batch + 2 + 2 * num_tokens, dtype=torch.int32, device=dev)
-    out = Slots(buf[:batch + 1], buf[2 * batch + 2:2 * batch + 2 + num_tokens],
-                buf[2 * batch + 2 + num_tokens:], buf[batch + 1:2 * batch + 1],
-                buf[2 * batch + 1:2 * batch + 2])
-    base = buf.data_ptr()
+    sizes = (batch + 1, num_tokens, num_tokens, batch, 1)
+    buf = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
+    out = Slots(*buf.split_with_sizes(sizes))
+    cu = buf.data_ptr()
+    pos = cu + 4 * (batch + 1)
+    slots = pos + 4 * num_tokens
+    lens = slots + 4 * num_tokens
     _call("pi0_build_slots", dev, batch, kv_lens.data_ptr(), new_lens.data_ptr(),
           block_table.data_ptr(), max(block_table.stride(0), max_pages), max_pages,
           free_pages.data_ptr(), free_pages.shape[0], free_pos.data_ptr(), num_pages, page_size,
-          num_tokens, base, base + 4 * (2 * batch + 2), base + 4 * (2 * batch + 2 + num_tokens),
-          base + 4 * (batch + 1), base + 4 * (2 * batch + 1), _err_ptr(err, dev))
+          num_tokens, cu, pos, slots, lens, lens + 4 * batch, _err_ptr(err, dev))
     return out
 
 
@@ -238,19 +269,15 @@ def write_kv(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torc
     code = _dtype(k, "k")
     dev = k.device
     c = _cache(cache, dev)
-    tokens = k.shape[0]
-    _rows(k, "k", dev, k.dtype, (tokens, c.kv_heads, c.head_dim))
-    _rows(v, "v", dev, k.dtype, (tokens, c.kv_heads, c.head_dim))
-    for t, name, n in ((cu_seqlens, "cu_seqlens", kv_lens.shape[0] + 1),
-                       (kv_lens, "kv_lens", kv_lens.shape[0]),
-                       (slot_mapping, "slot_mapping", tokens)):
-        _ints(t, name, dev, 1)
-        if t.shape[0] != n:
-            raise ValueError(f"{name} must hold {n} numbers")
+    tokens, batch = k.shape[0], kv_lens.shape[0]
+    shape = torch.Size((tokens, c.kv_heads, c.head_dim))
+    _ints(kv_lens, "kv_lens", dev, 1)
+    _ints(cu_seqlens, "cu_seqlens", dev, 1, batch + 1)
+    _ints(slot_mapping, "slot_mapping", dev, 1, tokens)
     if max_new is not None and max_new < 0:
         raise ValueError("max_new must not be negative")
-    _call("pi0_write_kv", dev, code, k.data_ptr(), *_strides(k), v.data_ptr(),
-          *_strides(v), tokens, kv_lens.shape[0], cu_seqlens.data_ptr(),
+    _call("pi0_write_kv", dev, code, *_rows(k, "k", dev, k.dtype, shape),
+          *_rows(v, "v", dev, k.dtype, shape), tokens, batch, cu_seqlens.data_ptr(),
           kv_lens.data_ptr(), slot_mapping.data_ptr(), tokens if max_new is None else max_new,
           ctypes.byref(c), _err_ptr(err, dev))
 
@@ -270,36 +297,26 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     dev = q.device
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q and k must be [tokens, heads, head_dim]")
-    tokens, heads, dim = q.shape
-    kv_heads = k.shape[1]
+    dtype, (tokens, heads, dim), (keys, kv_heads, k_dim) = q.dtype, q.shape, k.shape
     _head_dim(dim)
-    if kv_heads < 1 or heads % kv_heads:
-        raise ValueError(f"{heads} query heads cannot share {kv_heads} kv heads")
-    _rows(q, "q", dev, q.dtype)
-    _rows(k, "k", dev, q.dtype, (k.shape[0], kv_heads, dim))
-    _rows(v, "v", dev, q.dtype, k.shape)
+    if kv_heads < 1 or heads % kv_heads or k_dim != dim:
+        raise ValueError(f"{heads} query heads of {dim} cannot share {kv_heads} kv heads of {k_dim}")
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
     batch = cu_seqlens_q.shape[0] - 1
     if batch < 0 or (batch == 0 and tokens):
         raise ValueError("cu_seqlens_q must hold one number more than there are requests")
-    for t, name, n in ((cu_seqlens_q, "cu_seqlens_q", batch + 1),
-                       (cu_seqlens_k, "cu_seqlens_k", batch + 1),
-                       (prefix_lens, "prefix_lens", batch)):
-        if t is None:
-            continue
-        _ints(t, name, dev, 1)
-        if t.shape[0] != n:
-            raise ValueError(f"{name} must hold {n} numbers")
+    _ints(cu_seqlens_q, "cu_seqlens_q", dev, 1)
+    _ints(cu_seqlens_k, "cu_seqlens_k", dev, 1, batch + 1)
+    if prefix_lens is not None:
+        _ints(prefix_lens, "prefix_lens", dev, 1, batch)
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
-    else:
-        _rows(out, "out", dev, q.dtype, q.shape)
-    _call("pi0_attention_prompt", dev, code, q.data_ptr(), *_strides(q), k.data_ptr(),
-          *_strides(k), v.data_ptr(), *_strides(v), tokens, k.shape[0],
-          heads, kv_heads, dim, batch, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    _call("pi0_attention_prompt", dev, code, *_rows(q, "q", dev, dtype), *_rows(k, "k", dev, dtype),
+          *_rows(v, "v", dev, dtype, k.shape), tokens, keys, heads, kv_heads, dim, batch,
+          cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
           None if prefix_lens is None else prefix_lens.data_ptr(),
-          1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), *_strides(out),
+          dim ** -0.5 if scale is None else scale, *_rows(out, "out", dev, dtype, q.shape),
           _err_ptr(err, dev))
     return out
 
@@ -314,26 +331,24 @@ def attention_paged(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor,
     code = _dtype(q, "q")
     dev = q.device
     c = _cache(cache, dev)
-    _rows(q, "q", dev, q.dtype)
+    dtype = q.dtype
+    q_rows = _rows(q, "q", dev, dtype)
     batch, heads, dim = q.shape
-    if dim != c.head_dim or heads % c.kv_heads or heads < 1:
+    if dim != c.head_dim or heads < 1 or heads % c.kv_heads:
         raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {c.kv_heads} kv heads of "
                          f"{c.head_dim}")
-    _ints(block_table, "block_table", dev, 2)
-    _ints(kv_lens, "kv_lens", dev, 1)
-    if block_table.shape[0] != batch or kv_lens.shape[0] != batch or block_table.shape[1] < 1:
-        raise ValueError(f"block_table and kv_lens must hold {batch} requests")
-    if out is None:
-        out = torch.empty((batch, heads, dim), dtype=q.dtype, device=dev)
-    else:
-        _rows(out, "out", dev, q.dtype, q.shape)
+    _ints(block_table, "block_table", dev, 2, batch)
+    _ints(kv_lens, "kv_lens", dev, 1, batch)
     max_pages = block_table.shape[1]
-    ws = torch.empty(_workspace_bytes(dev, heads, c.kv_heads, dim, c.page_size), dtype=torch.uint8,
-                     device=dev)
-    _call("pi0_attention_paged", dev, code, q.data_ptr(), *_strides(q), batch, heads,
-          ctypes.byref(c), block_table.data_ptr(), max(block_table.stride(0), max_pages),
-          max_pages, kv_lens.data_ptr(), 1.0 / math.sqrt(dim) if scale is None else scale,
-          out.data_ptr(), *_strides(out), ws.data_ptr(), ws.numel(), _err_ptr(err, dev))
+    if max_pages < 1:
+        raise ValueError("block_table must have a column")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ws = _workspace(dev, heads, c.kv_heads, dim, c.page_size)
+    _call("pi0_attention_paged", dev, code, *q_rows, batch, heads, ctypes.byref(c),
+          block_table.data_ptr(), max(block_table.stride(0), max_pages), max_pages,
+          kv_lens.data_ptr(), dim ** -0.5 if scale is None else scale,
+          *_rows(out, "out", dev, dtype, q.shape), ws.data_ptr(), ws.numel(), _err_ptr(err, dev))
     return out
 
 
