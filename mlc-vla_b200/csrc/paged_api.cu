@@ -173,6 +173,7 @@ int run_paged(const DecodeArgs& a, int device, int sms, cudaStream_t st) {
   const int group = a.heads / c.kv_heads;
   const int64_t most = (int64_t)a.batch * c.kv_heads * ((group + NH - 1) / NH) *
                        (((int64_t)a.max_pages * c.page_size + kDecTile - 1) / kDecTile);
+  if (most > INT_MAX) return PI0_ERR_UNSUPPORTED;
   const int ctas = (int)std::min<int64_t>((int64_t)sms * C::OCC, most);
   paged_decode_kernel<T, HD, NH><<<ctas, kDecThreads, C::SMEM, st>>>(tk, tv, a);
   if (cudaGetLastError() != cudaSuccess) return PI0_ERR_CUDA;

@@ -136,17 +136,30 @@ struct DecMeta {
   int batch, head, heads, count;
 };
 
-// first tile of CTA i when `total` tiles are shared by `ctas`
-__device__ __forceinline__ int64_t share_begin(int64_t i, int64_t total, int ctas) {
-  return i * total / ctas;
-}
+// `total` tiles (below 2^31, which the host sees to) in shares of `each` or, the first `extra` ones,
+// one more; no share is empty, so fewer tiles than CTAs leave the last CTAs without one.
+struct DecShares {
+  int each, extra;
+  __device__ __forceinline__ DecShares(int total, int ctas) {
+    const int some = max(1, min(total, ctas));
+    each = total / some;
+    extra = total - each * some;
+  }
+  __device__ __forceinline__ int begin(int cta, int total) const {
+    return min(total, cta * each + min(cta, extra));
+  }
+  __device__ __forceinline__ int owner(int tile) const {
+    const int wide = extra * (each + 1);
+    return tile < wide ? tile / (each + 1) : extra + (tile - wide) / each;
+  }
+};
 
 // A CTA's tiles as pieces, each a run of tiles of one unit. Every role walks the same pieces.
 struct DecWalk {
   const DecodeArgs& a;
   int subs;            // units per request: kv heads × chunks of their heads
   int b, sub, t0;      // next tile
-  int64_t rem;         // tiles left
+  int rem;             // tiles left
   int n, nt, take;     // the piece: tokens and tiles of its unit, tiles taken
   __device__ __forceinline__ bool next() {
     if (rem <= 0) return false;
@@ -157,7 +170,7 @@ struct DecWalk {
       if (nt > 0) break;
       ++b;
     }
-    take = (int)min(rem, (int64_t)(nt - t0));
+    take = min(rem, nt - t0);
     return true;
   }
   __device__ __forceinline__ void done() {
@@ -211,8 +224,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
       p_full[2], pv_done[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ float s_red[2][4][NH], s_qa[NH], s_l[4][NH];
-  __shared__ int64_t s_scan[kDecThreads / 32], s_begin, s_end, s_total;
-  __shared__ int s_at[3];
+  __shared__ int s_scan[kDecThreads / 32], s_begin, s_total, s_at[3];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.heads / a.cache.kv_heads, chunks = (group + NH - 1) / NH;
   const int subs = a.cache.kv_heads * chunks;
@@ -247,43 +259,40 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
   {
     const int per = (a.batch + kDecThreads - 1) / kDecThreads;
     const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-    int64_t mine = 0;
+    int mine = 0;
     for (int b = b0; b < b1; ++b)
-      mine += (int64_t)(((int64_t)held_len(a, b, cta == 0) + kDecTile - 1) / kDecTile) * subs;
-    int64_t inc = mine;
+      mine += (int)(((int64_t)held_len(a, b, cta == 0) + kDecTile - 1) / kDecTile) * subs;
+    int inc = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t up = __shfl_up_sync(~0u, inc, d);
+      const int up = __shfl_up_sync(~0u, inc, d);
       if (lane >= d) inc += up;
     }
     if (lane == 31) s_scan[warp] = inc;
     __syncthreads();
-    int64_t before = inc - mine, total = 0;
+    int before = inc - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kDecThreads / 32; ++w) {
       if (w < warp) before += s_scan[w];
       total += s_scan[w];
     }
-    const int some = (int)min((int64_t)ctas, total);  // CTAs with tiles: no share is empty
-    const int64_t x0 = cta < some ? share_begin(cta, total, some) : total;
-    const int64_t x1 = cta < some ? share_begin(cta + 1, total, some) : total;
+    const int x0 = DecShares(total, ctas).begin(cta, total);
     if (tid == 0) {
       s_begin = x0;
-      s_end = x1;
       s_total = total;
     }
     if (x0 >= before && x0 < before + mine) {
-      int64_t x = x0 - before;
+      int x = x0 - before;
       int b = b0;
       for (;; ++b) {
         const int nt = (int)(((int64_t)held_len(a, b, false) + kDecTile - 1) / kDecTile);
-        if (x < (int64_t)nt * subs) {
+        if (x < nt * subs) {
           s_at[0] = b;
-          s_at[1] = (int)(x / nt);
-          s_at[2] = (int)(x % nt);
+          s_at[1] = x / nt;
+          s_at[2] = x % nt;
           break;
         }
-        x -= (int64_t)nt * subs;
+        x -= nt * subs;
       }
     }
     // requests without tokens: zeros
@@ -301,8 +310,9 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int64_t total = s_total;
-  DecWalk w{a, subs, s_at[0], s_at[1], s_at[2], s_end - s_begin, 0, 0, 0};
+  const int total = s_total;
+  const DecShares shares(total, ctas);
+  DecWalk w{a, subs, s_at[0], s_at[1], s_at[2], shares.begin(cta + 1, total) - s_begin, 0, 0, 0};
 
   if (warp == 0) {
     // ---- producer: one lane per box ----
@@ -425,28 +435,32 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     const uint32_t tlane = tmem + ((uint32_t)(q4 * 32) << 16);
     bool ok = true;
     int g = 0;
-    int64_t x = s_begin;
+    int x = s_begin;
     DecMeta meta{0, 0, 0, 0};
     while (w.next()) {
       const int kv = w.sub / chunks, h0 = kv * group + (w.sub % chunks) * NH;
       const int nh = min(NH, group - (w.sub % chunks) * NH);
       // q in three parts, a warp per head; every QK of the piece before has been read by now
-      for (int h = q4; h < NH; h += 4) {
-        constexpr int E = HD / 32;
+      constexpr int E = HD / 32;                    // entries of a row per lane
+      __align__(16) T qraw[NH / 4][E];
+#pragma unroll
+      for (int u = 0; u < NH / 4; ++u) {            // all rows of the warp are requested at once
+        const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.q_tok +
+                     (h0 + min(q4 + 4 * u, nh - 1)) * a.q_head + lane * E;
+        if constexpr (E == 8) *reinterpret_cast<uint4*>(qraw[u]) = *reinterpret_cast<const uint4*>(q);
+        else if constexpr (E == 4) *reinterpret_cast<uint2*>(qraw[u]) = *reinterpret_cast<const uint2*>(q);
+        else *reinterpret_cast<uint32_t*>(qraw[u]) = *reinterpret_cast<const uint32_t*>(q);
+      }
+#pragma unroll
+      for (int u = 0; u < NH / 4; ++u) {
+        const int h = q4 + 4 * u;
         float v[E];
-        if (h < nh) {
-          const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.q_tok + (h0 + h) * a.q_head +
-                       lane * E;
 #pragma unroll
-          for (int e = 0; e < E; ++e) v[e] = Tr<T>::f(q[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) v[e] = 0.f;
-        }
+        for (int e = 0; e < E; ++e) v[e] = h < nh ? Tr<T>::f(qraw[u][e]) : 0.f;
         float am = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) am = fmaxf(am, isfinite(v[e]) ? fabsf(v[e]) : 0.f);
-        am = warp_max(am);
+        am = warp_max_f32(am);
         // 2^k with am·2^-k in [128, 256); a row of zeros takes the smallest
         const int k = max((int)(__float_as_uint(am) >> 23) - 127, -100) - 7;
         const float inv = __uint_as_float((uint32_t)(127 - k) << 23);
@@ -625,17 +639,21 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
         page1 = page2;
         sc = sc1;
       }
-      // ---- the piece's sums ----
-      if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
-      ok = __all_sync(~0u, ok);
+      // ---- the piece's sums: l while the last P·V runs ----
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         const float sum = warp_sum(l[h]);
         if (lane == 0) s_l[q4][h] = sum;
       }
       named_sync<1, 128>();
+      float inv[NH];
 #pragma unroll
-      for (int h = 0; h < NH; ++h) l[h] = (s_l[0][h] + s_l[1][h]) + (s_l[2][h] + s_l[3][h]);
+      for (int h = 0; h < NH; ++h) {
+        l[h] = (s_l[0][h] + s_l[1][h]) + (s_l[2][h] + s_l[3][h]);
+        inv[h] = 1.f / (16.f * l[h]);
+      }
+      if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+      ok = __all_sync(~0u, ok);
       named_sync<1, 128>();  // s_l may be written again
       const bool whole = w.take == w.nt;
       float* part = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + (w.t0 > 0 ? 0 : 1)) * C::PARTIAL;
@@ -663,7 +681,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
             if (h >= nh) break;
             if (whole)
               reinterpret_cast<T*>(a.out)[w.b * a.o_tok + (h0 + h) * a.o_head + d] =
-                  Tr<T>::t(o[h] / (16.f * l[h]));
+                  Tr<T>::t(o[h] * inv[h]);
             else
               part[h * HD + d] = o[h];
           }
@@ -678,12 +696,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
             part[NH * HD + NH + h] = l[h];
           }
         if (w.t0 == 0) {
-          // the CTA of the unit's last tile
-          const int64_t last = x + w.nt - 1;
-          const int some = (int)min((int64_t)ctas, total);
-          int64_t e = last * some / total;
-          while (share_begin(e + 1, total, some) <= last) ++e;
-          meta = DecMeta{w.b, h0, nh, (int)(e - cta) + 1};
+          meta = DecMeta{w.b, h0, nh, shares.owner(x + w.nt - 1) - cta + 1};
         }
       }
       x += w.take;
@@ -712,15 +725,31 @@ __global__ void __launch_bounds__(HD) paged_join_kernel(DecodeArgs a, int ctas) 
   const float* first = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + 1) * C::PARTIAL;
   // partial i: slot 1 of the first CTA, slot 0 of those behind it
   auto part = [&](int i) { return first + (i == 0 ? 0 : ((size_t)i * 2 - 1) * C::PARTIAL); };
-  float M = -INFINITY;
-  for (int i = 0; i < meta.count; ++i) M = fmaxf(M, part(i)[NH * HD + h]);
-  float o = 0.f, l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < meta.count; ++i) {
-    const float* p = part(i);
-    const float f = exp2f(p[NH * HD + h] - M);
-    l = fmaf(f, p[NH * HD + NH + h], l);
-    o = fmaf(f, p[h * HD + d], o);
+  // eight partials at a time, so that their loads are in flight together
+  float M = -INFINITY, o = 0.f, l = 0.f;
+  for (int i0 = 0; i0 < meta.count; i0 += 8) {
+    float pm[8], pl[8], po[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool have = i0 + i < meta.count;
+      const float* p = part(have ? i0 + i : 0);
+      pm[i] = have ? p[NH * HD + h] : -INFINITY;
+      pl[i] = have ? p[NH * HD + NH + h] : 0.f;
+      po[i] = have ? p[h * HD + d] : 0.f;
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, pm[i]);
+    const float ref = top == -INFINITY ? 0.f : top, old = exp2f(M - ref);
+    o *= old;
+    l *= old;
+    M = top;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = exp2f(pm[i] - ref);
+      o = fmaf(f, po[i], o);
+      l = fmaf(f, pl[i], l);
+    }
   }
   reinterpret_cast<T*>(a.out)[meta.batch * a.o_tok + (meta.head + h) * a.o_head + d] =
       Tr<T>::t(o / (16.f * l));

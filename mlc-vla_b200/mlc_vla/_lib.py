@@ -1,15 +1,17 @@
 """Build and load ``libpi0b200.so`` (the sm_100a kernels behind include/pi0b200.h).
 
 ``build()`` compiles ``csrc/pi0_api.cu`` (the model path) and ``csrc/paged_api.cu`` (the
-text-generation operators) side by side in-tree with nvcc for ``sm_100a`` and links them;
-``load()`` opens the library with ctypes and declares every entry point of the header. There is no fallback: when
+text-generation operators) side by side in-tree with nvcc for ``sm_100a`` and links them, and
+``csrc/paged_bind.cpp``, the Python binding of the latter, with g++; ``load()`` opens the library with ctypes and declares every entry point of the header. There is no fallback: when
 the library is missing, ``load()`` raises.
 """
 
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
+import shutil
 import subprocess
 import threading
 
@@ -18,6 +20,7 @@ PROJECT_DIR = os.path.dirname(PKG_DIR)                      # mlc-vla_b200/
 CSRC_DIR = os.path.join(PROJECT_DIR, "csrc")
 INCLUDE_DIR = os.path.join(os.path.dirname(PROJECT_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libpi0b200.so")
+BIND_PATH = os.path.join(PKG_DIR, "lib", "_paged_native.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -50,9 +53,36 @@ EXPORTED = (
 )
 
 
+# the entry points behind the binding, in the order that it takes them
+PAGED = ("pi0_build_slots", "pi0_write_kv", "pi0_attention_prompt", "pi0_attention_paged",
+         "pi0_attention_paged_workspace")
+
+
 def _sources():
     return [os.path.join(CSRC_DIR, f) for f in sorted(os.listdir(CSRC_DIR))
             if f.endswith((".cu", ".cuh", ".h"))] + [os.path.join(INCLUDE_DIR, "pi0b200.h")]
+
+
+_BIND_SOURCES = [os.path.join(CSRC_DIR, "paged_bind.cpp"), os.path.join(INCLUDE_DIR, "pi0b200.h")]
+
+
+def _bind_command(out: str):
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    nvcc = shutil.which("nvcc")
+    cuda = os.environ.get("CUDA_HOME") or (os.path.dirname(os.path.dirname(os.path.realpath(nvcc)))
+                                           if nvcc else "/usr/local/cuda")
+    include = [INCLUDE_DIR, os.path.join(root, "include"),
+               os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            *(f"-I{d}" for d in include), _BIND_SOURCES[0], "-o", out,
+            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+            "-lc10_cuda"]
 
 
 def _unit_sources(unit: str):
@@ -71,7 +101,7 @@ def _stale(target: str, sources) -> bool:
 
 
 def needs_build() -> bool:
-    return _stale(LIB_PATH, _sources())
+    return _stale(LIB_PATH, _sources()) or _stale(BIND_PATH, _BIND_SOURCES)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -80,6 +110,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB_PATH
     os.makedirs(os.path.dirname(LIB_PATH), exist_ok=True)
     objects, running = [], []
+    if force or _stale(BIND_PATH, _BIND_SOURCES):
+        cmd = _bind_command(BIND_PATH + ".tmp")
+        if verbose:
+            print(" ".join(cmd))
+        running.append((BIND_PATH, cmd, subprocess.Popen(cmd, cwd=CSRC_DIR)))
     for unit in UNITS:
         obj = os.path.join(os.path.dirname(LIB_PATH), unit.replace(".cu", ".o"))
         objects.append(obj)
@@ -144,6 +179,7 @@ class Pi0Kv8C(ctypes.Structure):
 
 
 _lib = None
+_native = None
 _lock = threading.Lock()
 
 
@@ -220,6 +256,29 @@ def load():
         del fp
         _lib = lib
         return lib
+
+
+def load_paged():
+    """The binding of the text-generation operators, on the entry points of ``load()``'s library.
+    Raises if it was not built."""
+    global _native
+    if _native is not None:
+        return _native
+    lib = load()
+    with _lock:
+        if _native is None:
+            import torch  # noqa: F401  the binding's own libraries
+
+            if not os.path.exists(BIND_PATH):
+                raise RuntimeError(f"{BIND_PATH} is missing: build it with `python -c 'import "
+                                   f"mlc_vla._lib as l; l.build()'`.")
+            spec = importlib.util.spec_from_file_location("_paged_native", BIND_PATH)
+            native = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(native)
+            native.raise_status_with(Pi0Error)
+            native.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in PAGED))
+            _native = native
+    return _native
 
 
 class Pi0Error(RuntimeError):
