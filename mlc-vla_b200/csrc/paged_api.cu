@@ -244,13 +244,26 @@ int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_hea
       !cu_seqlens || !kv_lens || !slot_mapping)
     return PI0_ERR_INVALID;
   if (batch > 65535 || cache->kv_heads > 32767) return PI0_ERR_UNSUPPORTED;
+  // as many vectors a lane, then as many warps, as hold a (page, kv head) in registers
+  const int64_t vecs = (int64_t)std::min(cache->page_size, std::min(max_new, num_tokens)) *
+                       (cache->head_dim / 8);
+  const int held = vecs <= 32 ? 1 : vecs <= 128 ? 4 : 16;
+  int warps = 1;
+  while (warps < kWriteWarps && vecs > (int64_t)warps * 32 * held) warps *= 2;
   WriteArgs a{{k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride},
-              cu_seqlens, kv_lens, slot_mapping, err, cache_of(cache), num_tokens};
+              cu_seqlens, kv_lens, slot_mapping, err, cache_of(cache), num_tokens, warps};
   // n tokens touch at most ⌈(n − 1)/page⌉ + 1 pages; a request with more than max_new loops
-  const int pages = (std::min(max_new, num_tokens) + cache->page_size - 2) / cache->page_size + 1;
-  const dim3 grid(pages, 2 * cache->kv_heads, batch);
-  if (dtype == PI0_F16) write_kv_kernel<__half><<<grid, kWriteThreads, 0, stream>>>(a);
-  else write_kv_kernel<__nv_bfloat16><<<grid, kWriteThreads, 0, stream>>>(a);
+  const int64_t pages = (std::min(max_new, num_tokens) + (int64_t)cache->page_size - 2) /
+                            cache->page_size + 1;
+  const int units = kWriteWarps / warps;
+  const int64_t blocks = (pages * 2 * cache->kv_heads + units - 1) / units;
+  const dim3 grid((unsigned)std::min<int64_t>(blocks, INT_MAX), 1, batch);
+  const int threads = 32 * kWriteWarps;
+  auto go = [&](auto kernel) { kernel<<<grid, threads, 0, stream>>>(a); };
+  const bool half = dtype == PI0_F16;
+  if (held == 1) go(half ? write_kv_kernel<__half, 1> : write_kv_kernel<__nv_bfloat16, 1>);
+  else if (held == 4) go(half ? write_kv_kernel<__half, 4> : write_kv_kernel<__nv_bfloat16, 4>);
+  else go(half ? write_kv_kernel<__half, 16> : write_kv_kernel<__nv_bfloat16, 16>);
   return launched();
 }
 

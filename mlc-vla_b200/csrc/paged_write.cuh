@@ -7,7 +7,10 @@
 // new step (exact for every code that stays above e4m3's subnormals). An infinity or a NaN has no
 // finite code: it is stored as NaN and does not count for the scale.
 //
-// Bound by HBM: 2 bytes read and 1 written per element, plus the scales.
+// Bound by HBM: 2 bytes read and 1 written per element, plus the scales. A (page, kv head) is held in
+// the registers of the few warps that take it, up to 16 vectors of 16 bytes a lane: one pass over the
+// data, whose loads are all in flight before the first is used, and no wait but one between those
+// warps. Larger pages are read twice.
 #pragma once
 
 #include "paged_common.cuh"
@@ -15,7 +18,7 @@
 namespace pi0 {
 namespace paged {
 
-constexpr int kWriteThreads = 128;
+constexpr int kWriteWarps = 8;
 
 struct WriteArgs {
   const void* x[2];          // keys, values: [tokens, kv heads, head_dim], last dimension contiguous
@@ -26,6 +29,7 @@ struct WriteArgs {
   int* err;
   Cache cache;
   int tokens;
+  int warps;                 // per (page, kv head, key or value): 1, 2, 4 or 8
 };
 
 // smallest power of two s ≥ 2^-64 with amax ≤ 448·s: amax = f·2^e with f in [1, 2), 448 = 1.75·2^8
@@ -36,82 +40,163 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float((uint32_t)(max(x, -64) + 127) << 23);
 }
 
-__device__ __forceinline__ uint16_t to_e4m3x2(float a, float b) {
-  if (isinf(a)) a = NAN;
-  if (isinf(b)) b = NAN;
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+// codes of eight values times `inv`; an infinity (only where `odd`) becomes NaN, as it has no code
+__device__ __forceinline__ uint2 to_e4m3x8(const float (&v)[8], float inv, bool odd) {
+  __align__(8) uint16_t o[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    float x = v[2 * u] * inv, y = v[2 * u + 1] * inv;
+    if (odd) {
+      if (isinf(x)) x = NAN;
+      if (isinf(y)) y = NAN;
+    }
+    o[u] = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+  }
+  return *reinterpret_cast<uint2*>(o);
 }
 
-// One block per (page that the request's new tokens touch, kv head, key or value).
 template <typename T>
-__global__ void __launch_bounds__(kWriteThreads) write_kv_kernel(WriteArgs a) {
-  const int r = blockIdx.z, h = blockIdx.y >> 1, kind = blockIdx.y & 1;
+__device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = Tr<T>::f(e[i]);
+}
+
+// Magnitudes of 16-bit floats order like their bits below the sign, so the largest of a vector is an
+// integer maximum of pairs; from the type's infinity up they are no numbers.
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, uint4 v) {
+  m = __vmaxu2(m, v.x & 0x7fff7fffu);
+  m = __vmaxu2(m, v.y & 0x7fff7fffu);
+  m = __vmaxu2(m, v.z & 0x7fff7fffu);
+  return __vmaxu2(m, v.w & 0x7fff7fffu);
+}
+// the same, of the numbers only
+__device__ __forceinline__ uint32_t max_bits_finite(uint32_t m, uint4 v, uint32_t inf) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
+    m = __vmaxu2(m, (lo < inf ? lo : 0u) | (hi < inf ? hi << 16 : 0u));
+  }
+  return m;
+}
+
+// VECS: vectors a lane holds
+template <typename T, int VECS>
+__global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_kernel(WriteArgs a) {
+  constexpr uint32_t kInf = Tr<T>::kBf16 ? 0x7f80u : 0x7c00u;
   const Cache& c = a.cache;
-  const int ps = c.page_size, hd = c.head_dim, vec = hd / 8;
-  const int tid = threadIdx.x;
-  __shared__ float s_max[kWriteThreads / 32];
+  const int ps = c.page_size, hd = c.head_dim, vec = hd / 8, kinds = 2 * c.kv_heads;
+  const int lanes = 32 * a.warps, units = kWriteWarps / a.warps;  // of a unit, of a block
+  const int unit = threadIdx.x / lanes, g = threadIdx.x % lanes;
+  __shared__ uint32_t s_max[2][kWriteWarps];
+  const int r = blockIdx.z;
   const int start = max(a.kv_lens[r], 0);
   const int t0 = min(max(a.cu[r], 0), a.tokens), t1 = min(max(a.cu[r + 1], t0), a.tokens);
   if (t1 == t0) return;
   const int64_t end = (int64_t)start + (t1 - t0);
   const int p0 = start / ps, pages = (int)((end - 1) / ps) - p0 + 1;
-  const T* x = reinterpret_cast<const T*>(a.x[kind]) + h * a.head_stride[kind];
-  for (int j = blockIdx.x; j < pages; j += gridDim.x) {
+  // the warps of a unit meet at a barrier of their own
+  auto meet = [&]() {
+    if (a.warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + unit), "r"(lanes) : "memory");
+  };
+  auto reduce = [&](uint32_t m, int slot) -> uint32_t {
+    m = __reduce_max_sync(~0u, max(m & 0xffffu, m >> 16));
+    if (a.warps > 1) {
+      if ((threadIdx.x & 31) == 0) s_max[slot][threadIdx.x >> 5] = m;
+      meet();
+      for (int w = 0; w < a.warps; ++w) m = max(m, s_max[slot][unit * a.warps + w]);
+    }
+    return m;
+  };
+
+  // unit x of the request: page x / kinds, and head and kind x % kinds. Neighbours share tokens.
+  for (int64_t x = (int64_t)blockIdx.x * units + unit; x < (int64_t)pages * kinds;
+       x += (int64_t)gridDim.x * units) {
+    const int j = (int)(x / kinds), h = (int)(x % kinds) >> 1, kind = (int)(x % kinds) & 1;
     const int64_t lo = max((int64_t)start, (int64_t)(p0 + j) * ps);
     const int64_t hi = min(end, (int64_t)(p0 + j + 1) * ps);
     const int tok = t0 + (int)(lo - start), row = (int)(lo % ps), n = (int)(hi - lo);
+    const T* src = reinterpret_cast<const T*>(a.x[kind]) + tok * a.tok_stride[kind] +
+                   h * a.head_stride[kind];
+    // vector i of this lane is vector v = g + i·lanes of the unit, at (token, column) = (t, d)
+    const int nv = n * vec, dt = lanes / vec, dd = lanes % vec;
+    const int64_t tok_stride = a.tok_stride[kind];
+    auto at = [&](int v) { return src + (v / vec) * tok_stride + (v % vec) * 8; };
+    uint4 held[VECS];
+    {
+      int t = g / vec, d = g % vec;
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        held[i] = g + i * lanes < nv ? *reinterpret_cast<const uint4*>(src + t * tok_stride + d * 8)
+                                     : make_uint4(0, 0, 0, 0);
+        t += dt;
+        d += dd;
+        if (d >= vec) {
+          d -= vec;
+          ++t;
+        }
+      }
+    }
     const int slot = a.slots[tok];
-    if (slot < 0) continue;  // not admitted to the pool
     const int page = slot / ps;
-    if (page >= c.num_pages || slot % ps != row) {
-      if (tid == 0) set_err(a.err, PI0_PAGED_ERR_PAGE);
-      continue;
-    }
-    float am = 0.f;
-    for (int i = tid; i < n * vec; i += kWriteThreads) {
-      float v[8];
-      load8(x + (int64_t)(tok + i / vec) * a.tok_stride[kind] + (i % vec) * 8, v);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) am = fmaxf(am, isfinite(v[u]) ? fabsf(v[u]) : 0.f);
-    }
-    am = warp_max(am);
-    __syncthreads();  // s_max of the page before has been read
-    if ((tid & 31) == 0) s_max[tid >> 5] = am;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWriteThreads / 32; ++w) am = fmaxf(am, s_max[w]);
+    const bool none = slot < 0;  // not admitted to the pool
+    const bool bad = !none && (page >= c.num_pages || slot % ps != row);
+    if (bad && g == 0) set_err(a.err, PI0_PAGED_ERR_PAGE);
+    if (none || bad) continue;   // the same for all lanes of the unit
     const int64_t ph = (int64_t)page * c.kv_heads + h;
     float* sp = (kind ? c.vs : c.ks) + ph;
     uint8_t* codes = (kind ? c.v : c.k) + ph * ps * hd;
-    float s = pow2_scale(am);
+    const float old = row > 0 ? *sp : 0.f;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) m = max_bits(m, held[i]);
+#pragma unroll 1
+    for (int v = g + VECS * lanes; v < nv; v += lanes)
+      m = max_bits(m, *reinterpret_cast<const uint4*>(at(v)));
+    m = reduce(m, 0);
+    const bool odd = m >= kInf;
+    if (odd) {
+      m = 0;
+#pragma unroll 1
+      for (int v = g; v < nv; v += lanes)
+        m = max_bits_finite(m, *reinterpret_cast<const uint4*>(at(v)), kInf);
+      m = reduce(m, 1);
+    }
+    const uint16_t bits = (uint16_t)m;
+    float s = pow2_scale(Tr<T>::f(*reinterpret_cast<const T*>(&bits)));
     if (row > 0) {
-      const float old = *sp;
       if (old >= s) {
         s = old;
       } else {
         const float ratio = old / s;
-        for (int i = tid; i < row * vec; i += kWriteThreads) {
+        for (int i = g; i < row * vec; i += lanes) {
           float v[8];
-          load8(codes + (int64_t)i * 8, ratio, v);
-          uint16_t o[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) o[u] = to_e4m3x2(v[2 * u], v[2 * u + 1]);
-          *reinterpret_cast<uint2*>(codes + (int64_t)i * 8) = *reinterpret_cast<uint2*>(o);
+          load8(codes + (int64_t)i * 8, 1.f, v);
+          *reinterpret_cast<uint2*>(codes + (int64_t)i * 8) = to_e4m3x8(v, ratio, false);
         }
       }
     }
     const float inv = 1.f / s;
-    for (int i = tid; i < n * vec; i += kWriteThreads) {
-      float v[8];
-      load8(x + (int64_t)(tok + i / vec) * a.tok_stride[kind] + (i % vec) * 8, v);
-      __align__(8) uint16_t o[4];
+    uint8_t* dst = codes + (int64_t)row * hd;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) o[u] = to_e4m3x2(v[2 * u] * inv, v[2 * u + 1] * inv);
-      *reinterpret_cast<uint2*>(codes + (int64_t)row * hd + (int64_t)i * 8) =
-          *reinterpret_cast<uint2*>(o);
+    for (int i = 0; i < VECS; ++i) {
+      const int v = g + i * lanes;
+      if (v < nv) {
+        float f[8];
+        unpack8<T>(held[i], f);
+        *reinterpret_cast<uint2*>(dst + (int64_t)v * 8) = to_e4m3x8(f, inv, odd);
+      }
     }
-    __syncthreads();  // every thread has read the old scale
-    if (tid == 0) *sp = s;
+#pragma unroll 1
+    for (int v = g + VECS * lanes; v < nv; v += lanes) {
+      float f[8];
+      load8(at(v), f);
+      *reinterpret_cast<uint2*>(dst + (int64_t)v * 8) = to_e4m3x8(f, inv, odd);
+    }
+    meet();  // every lane has read the old scale, and s_max
+    if (g == 0) *sp = s;
   }
 }
 
