@@ -253,15 +253,19 @@ int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_hea
  * over the keys seen, fp32 softmax; a query that sees none, and a token of no request, give zeros.
  * Keys and values that a query does not see do not reach its result, whatever they hold. Head
  * sizes 64, 128 and 256 with up to 128 query heads per kv head run on tensor cores and need `err`,
- * which also takes the codes of bounded waits; the others need none. */
+ * which also takes the codes of bounded waits, and a workspace: 16-byte aligned, of the size that
+ * pi0_attention_prompt_workspace returns for the current device (-1: bad sizes or no device), for
+ * the sums of tiles that several CTAs share. Its contents before and after a call do not matter, but
+ * calls that may run at the same time need one each. The other sizes need neither. */
+int64_t pi0_attention_prompt_workspace(int heads, int kv_heads, int head_dim);
 int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const void* k, int64_t k_token_stride, int64_t k_head_stride,
                          const void* v, int64_t v_token_stride, int64_t v_head_stride,
                          int total_q, int total_k, int heads, int kv_heads, int head_dim,
                          int batch, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                          const int32_t* prefix_lens, float scale, void* out,
-                         int64_t o_token_stride, int64_t o_head_stride, int* err,
-                         pi0_stream_t stream);
+                         int64_t o_token_stride, int64_t o_head_stride, void* workspace,
+                         int64_t workspace_bytes, int* err, pi0_stream_t stream);
 
 /* Attention of one token per request over the cache: q, out [batch, heads, head_dim]; the request
  * sees its kv_lens[r] cached tokens (the new one's keys and values are written before the call).

@@ -103,7 +103,7 @@ int make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, const c
 // ---- attention over prompts -----------------------------------------------------------------
 
 template <typename T, int HD>
-int run_prompt(const PromptArgs& a, int device, cudaStream_t st) {
+int run_prompt(const PromptArgs& a, int device, int sms, cudaStream_t st) {
   using C = PromptCfg<HD>;
   constexpr CUtensorMapDataType type =
       Tr<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -122,20 +122,42 @@ int run_prompt(const PromptArgs& a, int device, cudaStream_t st) {
   if (!rc) rc = map(&tv, a.v, a.kv_heads, a.total_k, a.v_head, a.v_tok, 1, C::VKEYS);
   if (rc) return rc;
   if (!allow_smem<prompt_tc_kernel<T, HD>>(device, C::SMEM)) return PI0_ERR_CUDA;
-  // every request has at most one tile that is not full
+  // Steps at most: every request has at most one tile of queries that is not full, and no tile has
+  // more tiles of keys than there are.
   const int64_t tiles = (int64_t)a.total_q / (C::NQ * tok) + a.batch;
-  const int64_t grid = tiles * a.kv_heads;
-  if (grid > INT_MAX) return PI0_ERR_UNSUPPORTED;
-  prompt_tc_kernel<T, HD><<<(unsigned)grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, a, tok);
-  return launched();
+  const int64_t most = tiles * a.kv_heads * ((a.total_k + kKeys - 1) / kKeys);
+  const int ctas = (int)std::min<int64_t>(sms, most);
+  prompt_tc_kernel<T, HD><<<ctas, C::THREADS, C::SMEM, st>>>(tq, tk, tv, a, tok);
+  if (cudaGetLastError() != cudaSuccess) return PI0_ERR_CUDA;
+  if (a.total_k <= kKeys) return PI0_OK;  // a tile has one step: none is split
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, C::NQ * (HD / 32));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, prompt_join_kernel<T, HD>, a, tok, ctas) == cudaSuccess
+             ? PI0_OK : PI0_ERR_CUDA;
+}
+
+template <int HD>
+int64_t prompt_ws(int sms) {
+  return (int64_t)sms * (16 + 2 * PromptCfg<HD>::PARTIAL * (int64_t)sizeof(float));
+}
+
+bool prompt_tc(int heads, int kv_heads, int head_dim) {
+  return (head_dim == 64 || head_dim == 128 || head_dim == 256) && heads / kv_heads <= 128;
 }
 
 template <typename T>
-int run_prompt_any(const PromptArgs& a, int device, cudaStream_t st) {
+int run_prompt_any(const PromptArgs& a, int device, int sms, cudaStream_t st) {
   switch (a.head_dim) {
-    case 64: return run_prompt<T, 64>(a, device, st);
-    case 128: return run_prompt<T, 128>(a, device, st);
-    default: return run_prompt<T, 256>(a, device, st);
+    case 64: return run_prompt<T, 64>(a, device, sms, st);
+    case 128: return run_prompt<T, 128>(a, device, sms, st);
+    default: return run_prompt<T, 256>(a, device, sms, st);
   }
 }
 
@@ -267,14 +289,24 @@ int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_hea
   return launched();
 }
 
+int64_t pi0_attention_prompt_workspace(int heads, int kv_heads, int head_dim) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads) return -1;
+  if (!prompt_tc(heads, kv_heads, head_dim)) return 0;
+  int device;
+  const int sms = sm_count(&device);
+  if (!sms) return -1;
+  return head_dim == 64 ? prompt_ws<64>(sms) : head_dim == 128 ? prompt_ws<128>(sms)
+                                                               : prompt_ws<256>(sms);
+}
+
 int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const void* k, int64_t k_token_stride, int64_t k_head_stride,
                          const void* v, int64_t v_token_stride, int64_t v_head_stride,
                          int total_q, int total_k, int heads, int kv_heads, int head_dim,
                          int batch, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                          const int32_t* prefix_lens, float scale, void* out,
-                         int64_t o_token_stride, int64_t o_head_stride, int* err,
-                         pi0_stream_t stream) {
+                         int64_t o_token_stride, int64_t o_head_stride, void* workspace,
+                         int64_t workspace_bytes, int* err, pi0_stream_t stream) {
   if (!dtype_ok(dtype) || total_q < 0 || total_k < 0 || heads < 1 || kv_heads < 1 ||
       heads % kv_heads || head_dim < 8 || head_dim % 8 || head_dim > 256 || batch < 0)
     return PI0_ERR_INVALID;
@@ -288,15 +320,18 @@ int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64
   if (rows > INT_MAX) return PI0_ERR_UNSUPPORTED;
   PromptArgs a{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
                v_token_stride, v_head_stride, o_token_stride, o_head_stride, cu_seqlens_q,
-               cu_seqlens_k, prefix_lens, err, scale * 1.4426950408889634f, batch, total_q, total_k,
+               cu_seqlens_k, prefix_lens, err, static_cast<float*>(workspace),
+               scale * 1.4426950408889634f, batch, total_q, total_k,
                heads, kv_heads, head_dim};
-  if ((head_dim == 64 || head_dim == 128 || head_dim == 256) && heads / kv_heads <= 128 &&
-      total_k > 0) {
+  if (prompt_tc(heads, kv_heads, head_dim) && total_k > 0) {
     int device;
-    if (!err) return PI0_ERR_INVALID;
-    if (!sm_count(&device)) return PI0_ERR_CUDA;
-    return dtype == PI0_F16 ? run_prompt_any<__half>(a, device, stream)
-                            : run_prompt_any<__nv_bfloat16>(a, device, stream);
+    const int sms = sm_count(&device);
+    if (!sms) return PI0_ERR_CUDA;
+    if (!workspace || off16(workspace) || !err ||
+        workspace_bytes < pi0_attention_prompt_workspace(heads, kv_heads, head_dim))
+      return PI0_ERR_INVALID;
+    return dtype == PI0_F16 ? run_prompt_any<__half>(a, device, sms, stream)
+                            : run_prompt_any<__nv_bfloat16>(a, device, sms, stream);
   }
   const unsigned grid = (unsigned)((rows + kRowWarps - 1) / kRowWarps);
   if (dtype == PI0_F16) prompt_rows_kernel<__half><<<grid, 32 * kRowWarps, 0, stream>>>(a);

@@ -24,15 +24,19 @@ struct Entries {
   decltype(&pi0_write_kv) write_kv = nullptr;
   decltype(&pi0_attention_prompt) attention_prompt = nullptr;
   decltype(&pi0_attention_paged) attention_paged = nullptr;
+  decltype(&pi0_attention_prompt_workspace) attention_prompt_workspace = nullptr;
   decltype(&pi0_attention_paged_workspace) attention_paged_workspace = nullptr;
 } g_lib;
 
 void bind(uint64_t build_slots, uint64_t write_kv, uint64_t attention_prompt,
-          uint64_t attention_paged, uint64_t attention_paged_workspace) {
+          uint64_t attention_paged, uint64_t attention_prompt_workspace,
+          uint64_t attention_paged_workspace) {
   g_lib.build_slots = reinterpret_cast<decltype(g_lib.build_slots)>(build_slots);
   g_lib.write_kv = reinterpret_cast<decltype(g_lib.write_kv)>(write_kv);
   g_lib.attention_prompt = reinterpret_cast<decltype(g_lib.attention_prompt)>(attention_prompt);
   g_lib.attention_paged = reinterpret_cast<decltype(g_lib.attention_paged)>(attention_paged);
+  g_lib.attention_prompt_workspace =
+      reinterpret_cast<decltype(g_lib.attention_prompt_workspace)>(attention_prompt_workspace);
   g_lib.attention_paged_workspace =
       reinterpret_cast<decltype(g_lib.attention_paged_workspace)>(attention_paged_workspace);
 }
@@ -260,13 +264,17 @@ Tensor attention_prompt(const Tensor& q, const Tensor& k, const Tensor& v, const
   Tensor o = out ? *out : at::empty(q.sizes(), q.options());
   const Rows orr = rows(o, "out", dev, type);
   check_shape(o, "out", q.sizes());
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+  const int64_t bytes = g_lib.attention_prompt_workspace(fits32(heads, "heads"), (int)kv_heads, (int)dim);
+  if (bytes < 0) throw Status(PI0_ERR_CUDA, "pi0_attention_prompt_workspace");
+  const Tensor ws = workspace(dev, stream, bytes);
   check_status(g_lib.attention_prompt(code, qr.p, qr.tok, qr.head, kr.p, kr.tok, kr.head, vr.p,
                                       vr.tok, vr.head, fits32(tokens, "tokens"),
                                       fits32(k.size(0), "keys"), fits32(heads, "heads"),
                                       (int)kv_heads, (int)dim, fits32(batch, "requests"), cq, ck, pre,
                                       scale ? (float)*scale : 1.f / std::sqrt((float)dim), orr.p,
-                                      orr.tok, orr.head, err_of(err, dev),
-                                      c10::cuda::getCurrentCUDAStream(dev).stream()),
+                                      orr.tok, orr.head, ws.data_ptr(), ws.numel(),
+                                      err_of(err, dev), stream),
                "pi0_attention_prompt");
   return o;
 }

@@ -136,24 +136,6 @@ struct DecMeta {
   int batch, head, heads, count;
 };
 
-// `total` tiles (below 2^31, which the host sees to) in shares of `each` or, the first `extra` ones,
-// one more; no share is empty, so fewer tiles than CTAs leave the last CTAs without one.
-struct DecShares {
-  int each, extra;
-  __device__ __forceinline__ DecShares(int total, int ctas) {
-    const int some = max(1, min(total, ctas));
-    each = total / some;
-    extra = total - each * some;
-  }
-  __device__ __forceinline__ int begin(int cta, int total) const {
-    return min(total, cta * each + min(cta, extra));
-  }
-  __device__ __forceinline__ int owner(int tile) const {
-    const int wide = extra * (each + 1);
-    return tile < wide ? tile / (each + 1) : extra + (tile - wide) / each;
-  }
-};
-
 // A CTA's tiles as pieces, each a run of tiles of one unit. Every role walks the same pieces.
 struct DecWalk {
   const DecodeArgs& a;
@@ -276,7 +258,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
       if (w < warp) before += s_scan[w];
       total += s_scan[w];
     }
-    const int x0 = DecShares(total, ctas).begin(cta, total);
+    const int x0 = Shares<int>(total, ctas).begin(cta, total);
     if (tid == 0) {
       s_begin = x0;
       s_total = total;
@@ -311,7 +293,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int total = s_total;
-  const DecShares shares(total, ctas);
+  const Shares<int> shares(total, ctas);
   DecWalk w{a, subs, s_at[0], s_at[1], s_at[2], shares.begin(cta + 1, total) - s_begin, 0, 0, 0};
 
   if (warp == 0) {

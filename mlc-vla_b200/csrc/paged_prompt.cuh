@@ -20,6 +20,7 @@ struct PromptArgs {
   const int* cu_k;
   const int* prefix;   // or null: causal
   int* err;
+  float* ws;           // partials of the tensor-core form
   float c;             // logit scale · log2 e
   int batch, total_q, total_k, heads, kv_heads, head_dim;
 };
@@ -94,10 +95,88 @@ struct PromptCfg {
   static constexpr int VKEYS = kKeys / SPT;         // keys of a V slot
   // tensor memory: two tiles of logits, each overlaid by its weights, then the sums
   static constexpr int O_COL = 256;
+  // bytes of a row that a warp stages for output at a time: its 32 rows fit its part of a ring slot
+  static constexpr int STAGE = 64;
+  static_assert(4 * NQ * 32 * STAGE <= SLOT, "staged rows of all warps");
+  // a partial: for each tile of rows the sums as [HD / 4][128 rows][4], then M and l of the rows
+  static constexpr int PART_TILE = 128 * HD + 256;
+  static constexpr int PARTIAL = NQ * PART_TILE;
 };
 
-struct PromptTile {
-  int q0, lq, k0, lk, prefix, t0;
+// what a CTA leaves for the joining kernel about the tile that begins in it and goes on in others
+struct PromptMeta {
+  int request, tile, kv, count;
+};
+
+// A request, and the steps of its tiles: a step is a tile of query rows against a tile of keys.
+struct PromptSeq {
+  int q0, lq, k0, lk, prefix;
+  __device__ __forceinline__ void load(const PromptArgs& a, int b) {
+    seq_span(a.cu_q, b, a.total_q, q0, lq);
+    seq_span(a.cu_k, b, a.total_k, k0, lk);
+    prefix = a.prefix ? a.prefix[b] : 0;
+  }
+  __device__ __forceinline__ int sees(int i) const { return visible(i, lq, lk, prefix); }
+  // steps of the tile of queries [t0, t0 + span): its last query sees the most keys. A tile that
+  // sees none still takes one, which writes its zeros.
+  __device__ __forceinline__ int steps(int t0, int span) const {
+    return max(1, (sees(min(lq, t0 + span) - 1) + kKeys - 1) / kKeys);
+  }
+};
+
+// Writing a tile's rows takes about as long as a step, so in the shares a (tile, kv head) counts for
+// one more than its steps.
+constexpr int kTileCost = 1;
+
+// A CTA's steps as pieces, each a run of steps of one (tile, kv head). Every role walks the same.
+struct PromptWalk {
+  const PromptArgs& a;
+  int span;
+  int b, tile, kv, j0;  // next step: request, tile, kv head, tile of keys
+  int64_t at, end;      // its number, and the share's end
+  PromptSeq seq;
+  int nt, n, take;      // tiles of the request; steps of the piece's tile, steps taken
+  bool known;
+  __device__ __forceinline__ bool next() {
+    while (at < end) {
+      if (!known) {
+        for (;; ++b) {
+          if (b >= a.batch) return false;
+          seq.load(a, b);
+          nt = (seq.lq + span - 1) / span;
+          if (nt > 0) break;
+        }
+        known = true;
+      }
+      n = seq.steps(tile * span, span);
+      take = (int)min(end - at, (int64_t)(n - j0));
+      if (take > 0) return true;
+      done();  // the share begins behind the tile's last step
+    }
+    return false;
+  }
+  __device__ __forceinline__ void done() {
+    at += take;
+    j0 += take;
+    if (j0 < n) return;  // the share ends inside the tile
+    at += n + kTileCost - j0;
+    j0 = 0;
+    if (++kv < a.kv_heads) return;
+    kv = 0;
+    if (++tile < nt) return;
+    tile = 0;
+    ++b;
+    known = false;
+  }
+};
+
+
+// A piece, as the producer hands it to the other warps.
+struct __align__(16) PromptPiece {
+  int take, key0, fewest, first;   // steps (0: no more); first key; keys all its rows see; first query
+  int q0, lq, lk, prefix;          // its request
+  int kv, slot, count, request;    // whole: slot < 0, else of the CTA's partials; see PromptMeta
+  int k0, tile;
 };
 
 // largest of 128 logits, in four chains
@@ -110,7 +189,20 @@ __device__ __forceinline__ float max128(const float (&s)[128]) {
     c = max3(c, s[j + 4], s[j + 5]);
     d = max3(d, s[j + 6], s[j + 7]);
   }
-  return fmaxf(max3(a, s[124], s[125]), fmaxf(max3(b, s[126], s[127]), fmaxf(c, d)));
+  return fmaxf(max3(a, s[124], s[125]), max3(max3(b, s[126], s[127]), c, d));
+}
+
+// whether all softmax threads say so: they leave their loops together
+template <int NQ>
+__device__ __forceinline__ bool softmax_all(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, %2, p;\n"
+      " selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)v), "n"(NQ * 128)
+      : "memory");
+  return r != 0;
 }
 
 template <typename T, int HD>
@@ -119,18 +211,21 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                      const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, PromptArgs a, int tok) {
   using C = PromptCfg<HD>;
-  constexpr int NQ = C::NQ, SPT = C::SPT, SLOTS = C::SLOTS;
+  constexpr int NQ = C::NQ, SPT = C::SPT, SLOTS = C::SLOTS, WARPS = C::THREADS / 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = base + SLOTS * C::SLOT;
-  __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, s_full[2],
+  __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, q_empty, s_full[2],
       p_full[2][2], pv_done[2], drain;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_scan[C::THREADS / 32], s_req, s_tile, s_bad;
+  __shared__ int s_tiles[C::THREADS], s_scan[WARPS], s_at[4], s_bad;
+  __shared__ int64_t s_steps[WARPS], s_begin, s_total;
+  __shared__ PromptPiece s_piece[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kv = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
-  const int group = a.heads / a.kv_heads;
+  const int group = a.heads / a.kv_heads, span = NQ * tok;
+  const int ctas = gridDim.x, cta = blockIdx.x;
+  pdl_trigger();  // every CTA of this grid is resident at once: the joining blocks may queue up
 
   if (tid == 0) {
     for (int i = 0; i < SLOTS; ++i) {
@@ -138,6 +233,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       mbar_init(&empty[i], NQ);
     }
     mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 2 * NQ);  // its QKs are done, and the softmax warps have begun it
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i][0], 4);
@@ -149,19 +245,27 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-    s_req = -1;
     s_bad = 0x7fffffff;
   }
-  // ---- which tile: the tiles of the requests are numbered in order; `index` lies in one of them
-  const int span = NQ * tok;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&s_tmem)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+
+  // ---- this CTA's share of the steps ----
   {
+    // tiles before each thread's requests
     const int per = (a.batch + C::THREADS - 1) / C::THREADS;
     const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-    int mine = 0, t0, n;
-    for (int b = b0; b < b1; ++b) {
+    auto tiles_of = [&](int b) {
+      int t0, n;
       seq_span(a.cu_q, b, a.total_q, t0, n);
-      mine += (n + span - 1) / span;
-    }
+      return (n + span - 1) / span;
+    };
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(b);
     int inc = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -170,159 +274,216 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
     }
     if (lane == 31) s_scan[warp] = inc;
     __syncthreads();
-    int before = inc - mine;
+    int before = inc - mine, tiles = 0;
 #pragma unroll
-    for (int w = 0; w < C::THREADS / 32; ++w)
+    for (int w = 0; w < WARPS; ++w) {
       if (w < warp) before += s_scan[w];
-    if (index >= before && index < before + mine) {
-      int x = index - before;
-      for (int b = b0;; ++b) {
-        seq_span(a.cu_q, b, a.total_q, t0, n);
-        const int nt = (n + span - 1) / span;
-        if (x < nt) {
-          s_req = b;
-          s_tile = nt - 1 - x;  // the last tile of a request sees the most keys: first
+      tiles += s_scan[w];
+    }
+    s_tiles[tid] = before;
+    __syncthreads();
+    // steps before each thread's tiles
+    const int each = (tiles + C::THREADS - 1) / C::THREADS;
+    const int g0 = min(tiles, tid * each), g1 = min(tiles, g0 + each);
+    PromptSeq seq;
+    int b = 0, t = 0, nt = 0;        // request and tile of g0
+    if (g0 < g1) {
+      int lo = 0, hi = C::THREADS;   // the last thread whose requests start at or before tile g0
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_tiles[mid] <= g0) lo = mid; else hi = mid;
+      }
+      t = g0 - s_tiles[lo];
+      for (b = lo * per; t >= (nt = tiles_of(b)); ++b) t -= nt;
+      seq.load(a, b);
+    }
+    const int bg = b, tg = t;
+    int64_t sum = 0;
+    auto steps_of_next = [&]() {     // what tile (b, t) counts for, and on to the one behind it
+      while (t >= nt) {
+        t = 0;
+        nt = tiles_of(++b);
+        if (nt > 0) seq.load(a, b);
+      }
+      return seq.steps(t++ * span, span) + kTileCost;
+    };
+    for (int g = g0; g < g1; ++g) sum += steps_of_next();
+    sum *= a.kv_heads;
+    int64_t incs = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(~0u, incs, d);
+      if (lane >= d) incs += up;
+    }
+    if (lane == 31) s_steps[warp] = incs;
+    __syncthreads();
+    int64_t first = incs - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) first += s_steps[w];
+      total += s_steps[w];
+    }
+    const int64_t x0 = Shares<int64_t>(total, ctas).begin(cta, total);
+    if (tid == 0) {
+      s_begin = x0;
+      s_total = total;
+    }
+    if (x0 >= first && x0 < first + sum) {
+      int64_t x = x0 - first;
+      b = bg;
+      t = tg;
+      if (g0 < g1) {
+        nt = tiles_of(b);
+        seq.load(a, b);
+      }
+      for (;;) {
+        const int n = steps_of_next();
+        if (x < (int64_t)n * a.kv_heads) {
+          s_at[0] = b;
+          s_at[1] = t - 1;
+          s_at[2] = (int)x / n;
+          s_at[3] = (int)x % n;
           break;
         }
-        x -= nt;
+        x -= (int64_t)n * a.kv_heads;
       }
     }
     // tokens of no request: zeros
-    if (index == 0 && kv == 0) {
-      const int first = min(max(a.cu_q[0], 0), a.total_q);
-      const int behind = min(max(a.cu_q[a.batch], first), a.total_q);
-      const int64_t none = (int64_t)(first + a.total_q - behind) * a.heads * (HD / 8);
-      for (int64_t i = tid; i < none; i += C::THREADS) {
-        const int64_t row = i / (HD / 8);
-        int t = (int)(row / a.heads);
-        t = t < first ? t : behind + t - first;
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + t * a.o_tok +
-                                  (row % a.heads) * a.o_head + (i % (HD / 8)) * 8) =
-            make_uint4(0, 0, 0, 0);
-      }
+    const int head = min(max(a.cu_q[0], 0), a.total_q);
+    const int tail = min(max(a.cu_q[a.batch], head), a.total_q);
+    const int64_t none = (int64_t)(head + a.total_q - tail) * a.heads * (HD / 8);
+    for (int64_t i = (int64_t)cta * C::THREADS + tid; i < none; i += (int64_t)ctas * C::THREADS) {
+      const int64_t row = i / (HD / 8);
+      int tk = (int)(row / a.heads);
+      tk = tk < head ? tk : tail + tk - head;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + tk * a.o_tok +
+                                (row % a.heads) * a.o_head + (i % (HD / 8)) * 8) =
+          make_uint4(0, 0, 0, 0);
     }
-  }
-  __syncthreads();
-  if (s_req < 0) return;  // the grid is an upper bound of the tiles
-  PromptTile p;
-  seq_span(a.cu_q, s_req, a.total_q, p.q0, p.lq);
-  seq_span(a.cu_k, s_req, a.total_k, p.k0, p.lk);
-  p.prefix = a.prefix ? a.prefix[s_req] : 0;
-  p.t0 = s_tile * span;
-  // keys that the tile's last query sees, the most; and its first, the fewest
-  const int most = visible(min(p.lq, p.t0 + span) - 1, p.lq, p.lk, p.prefix);
-  const int fewest = visible(p.t0, p.lq, p.lk, p.prefix);
-  const int n = (most + kKeys - 1) / kKeys;
-
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(&s_tmem)),
-                 "r"(512u));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  // position of a tile's K or V in the order of the loads, in units of SPT slots: the order in
-  // which the MMAs take them
-  auto k_unit = [&](int j) { return NQ == 2 ? 2 * j : (j == 0 ? 0 : 2 * j - 1); };
-  auto v_unit = [&](int j) { return NQ == 2 ? 2 * j + 1 : min(2 * j + 2, n + j); };
+  const int64_t total = s_total;
+  const Shares<int64_t> shares(total, ctas);
+  // Position of the K or V of a piece's step j (of n) in the order of the loads, in units of SPT
+  // slots: the order in which the MMAs take them.
+  auto k_unit = [](int j) { return NQ == 2 ? 2 * j : (j == 0 ? 0 : 2 * j - 1); };
+  auto v_unit = [](int j, int n) { return NQ == 2 ? 2 * j + 1 : min(2 * j + 2, n + j); };
 
   // A row whose sum meets an infinity or a NaN may owe it to a value that it does not see (weight
-  // zero times infinity): then the CTA does its tile once more, with such values taken out of the
-  // V tiles that some of its rows see in part.
-  //
+  // zero times infinity): then the CTA does its share once more, with such values taken out of the
+  // V tiles that some rows of a piece see in part.
   // A row of 128 logits takes more registers than 1/12 of an SM's: where there are twelve warps, the
   // first warpgroup gives some of its own. (80 + 2·208)·128 of the 168·384 that the block was
   // launched with.
   if (warp < 4) {
-   if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-   for (int pass = 0; pass < 2; ++pass) {
-    const int load0 = pass * 2 * n * SPT, job0 = pass * NQ * n;
-    if (warp == 0) {
-      if (lane == 0 && n > 0) {
-        // ---- producer ----
-        bool ok = true;
-        int load = load0;
-        if (pass == 0) {
-          // bytes of whole boxes: what lies out of bounds arrives as zeros
-          mbar_expect_tx(&q_full, (uint32_t)(NQ * HD / 64 * tok * group * 128));
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    int done = 0, pieces = 0;  // steps and pieces so far
+    bool ok = true;
+    for (int pass = 0; pass < 2; ++pass) {
+      if (warp == 0) {
+        if (lane == 0) {
+          // ---- producer ----
+          PromptWalk w{a, span, s_at[0], s_at[1], s_at[2], s_at[3], s_begin,
+                       shares.begin(cta + 1, total), PromptSeq{}, 0, 0, 0, false};
+          int load = done * 2 * SPT;
+          auto slot_of = [&]() -> uint8_t* {
+            const int s = load % SLOTS;
+            if (load >= SLOTS)
+              ok = ok &&
+                   bar_wait(&empty[s], (load / SLOTS - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
+            if (!ok) return nullptr;
+            mbar_expect_tx(&full[s], C::SLOT);
+            ++load;
+            return base + s * C::SLOT;
+          };
+          auto load_k = [&](int j) {
+#pragma unroll 1
+            for (int h = 0; h < SPT; ++h) {
+              uint8_t* dst = slot_of();
+              if (!dst) return;
+              uint64_t* bar = &full[(load - 1) % SLOTS];
 #pragma unroll
-          for (int q = 0; q < NQ; ++q)
+              for (int kb = 0; kb < HD / 64 / SPT; ++kb)
+                tma_load_3d(dst + kb * 16384, &tmK, bar, (h * (HD / 64 / SPT) + kb) * 64, w.kv,
+                            w.seq.k0 + (w.j0 + j) * kKeys);
+            }
+          };
+          auto load_v = [&](int j) {
+#pragma unroll 1
+            for (int h = 0; h < SPT; ++h) {
+              uint8_t* dst = slot_of();
+              if (!dst) return;
+              uint64_t* bar = &full[(load - 1) % SLOTS];
 #pragma unroll
-            for (int kb = 0; kb < HD / 64; ++kb)
-              tma_load_3d(sQ + q * C::Q_TILE + kb * 16384, &tmQ, &q_full, kb * 64, kv * group,
-                          p.q0 + p.t0 + q * tok);
+              for (int kb = 0; kb < HD / 64; ++kb)
+                tma_load_3d(dst + kb * (C::VKEYS * 128), &tmV, bar, kb * 64, w.kv,
+                            w.seq.k0 + (w.j0 + j) * kKeys + h * C::VKEYS);
+            }
+          };
+          for (;;) {
+            const bool more = ok && w.next();
+            if (more) load_k(0);
+            // the piece before has been begun, and its QKs have read Q
+            if (ok && pieces > 0)
+              ok = bar_wait(&q_empty, (pieces - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
+            if (!ok) break;
+            PromptPiece& pc = s_piece[pieces & 1];
+            if (!more) {
+              pc.take = 0;
+              mbar_arrive(&q_full);
+              ++pieces;
+              break;
+            }
+            const bool whole = w.take == w.n;
+            pc = PromptPiece{w.take, w.j0 * kKeys, w.seq.sees(w.tile * span), w.tile * span,
+                             w.seq.q0, w.seq.lq, w.seq.lk, w.seq.prefix,
+                             w.kv, whole ? -1 : w.j0 > 0 ? 0 : 1,
+                             !whole && w.j0 == 0 ? shares.owner(w.at + w.n - 1) - cta + 1 : 0, w.b,
+                             w.seq.k0, w.tile};
+            // bytes of whole boxes: what lies out of bounds arrives as zeros
+            mbar_expect_tx(&q_full, (uint32_t)(NQ * HD / 64 * tok * group * 128));
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+              for (int kb = 0; kb < HD / 64; ++kb)
+                tma_load_3d(sQ + q * C::Q_TILE + kb * 16384, &tmQ, &q_full, kb * 64, w.kv * group,
+                            w.seq.q0 + w.tile * span + q * tok);
+            ++pieces;
+#pragma unroll 1
+            for (int j = 0; j < w.take && ok; ++j) {
+              if (NQ == 2 ? j > 0 : j + 1 < w.take) load_k(NQ == 2 ? j : j + 1);
+              if (ok) load_v(j);
+            }
+            done += w.take;
+            w.done();
+          }
+          // no copy into this CTA's shared memory may be in flight when it exits
+          if (ok)
+            bar_wait(&q_full, (pieces - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
+          for (int l = max(0, load - SLOTS); l < load; ++l)
+            bar_wait(&full[l % SLOTS], (l / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
         }
-        auto slot_of = [&]() -> uint8_t* {
-          const int s = load % SLOTS;
-          if (load >= SLOTS)
-            ok = ok && bar_wait(&empty[s], (load / SLOTS - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
-          if (!ok) return nullptr;
-          mbar_expect_tx(&full[s], C::SLOT);
-          ++load;
-          return base + s * C::SLOT;
-        };
-        auto load_k = [&](int j) {
-#pragma unroll
-          for (int h = 0; h < SPT; ++h) {
-            uint8_t* dst = slot_of();
-            if (!dst) return;
-            uint64_t* bar = &full[(load - 1) % SLOTS];
-#pragma unroll
-            for (int kb = 0; kb < HD / 64 / SPT; ++kb)
-              tma_load_3d(dst + kb * 16384, &tmK, bar, (h * (HD / 64 / SPT) + kb) * 64, kv,
-                          p.k0 + j * kKeys);
-          }
-        };
-        auto load_v = [&](int j) {
-#pragma unroll
-          for (int h = 0; h < SPT; ++h) {
-            uint8_t* dst = slot_of();
-            if (!dst) return;
-            uint64_t* bar = &full[(load - 1) % SLOTS];
-#pragma unroll
-            for (int kb = 0; kb < HD / 64; ++kb)
-              tma_load_3d(dst + kb * (C::VKEYS * 128), &tmV, bar, kb * 64, kv,
-                          p.k0 + j * kKeys + h * C::VKEYS);
-          }
-        };
-        if constexpr (NQ == 2) {
-          for (int j = 0; j < n && ok; ++j) {
-            load_k(j);
-            if (ok) load_v(j);
-          }
-        } else {
-          load_k(0);
-          for (int j = 0; j < n && ok; ++j) {
-            if (j + 1 < n) load_k(j + 1);
-            if (ok) load_v(j);
-          }
-        }
-        // no copy into this CTA's shared memory may be in flight when it exits
-        bar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
-        for (int l = max(load0, load - SLOTS); l < load; ++l)
-          bar_wait(&full[l % SLOTS], (l / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
-      }
-      __syncwarp();
-    } else if (warp <= NQ) {
-      if (n > 0) {
+        __syncwarp();
+      } else if (warp <= NQ) {
         // ---- MMA issuers: with two tiles of rows a warp for each, so that neither waits for the
         // other's weights. A tile's logits and weights share their columns, and MMAs of one thread
         // run in order: P·V j, then the logits that overwrite P.
         constexpr uint32_t id_s = tc::idesc_f16<T>(128, kKeys);
         constexpr uint32_t id_o = tc::idesc_f16<T>(128, HD) | (1u << 16);  // V is MN-major
+        constexpr int kAhead = NQ == 2 ? 1 : 2;  // steps whose logits come before the first weights
         const int q = warp - 1;
+        int take = 0;
         const uint32_t ring = __shfl_sync(~0u, smem_u32(base), 0), tm = __shfl_sync(~0u, tmem, 0);
         const uint32_t qs = ring + SLOTS * C::SLOT + q * C::Q_TILE, to = tm + C::O_COL + q * HD;
-        bool ok = bar_wait(&q_full, 0, a.err, tc::ERR_TIMEOUT_MMA);
         auto full_of = [&](int load) {
           return bar_wait(&full[load % SLOTS], (load / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
         };
-        auto job_of = [&](int j) { return job0 + (NQ == 2 ? 2 * j + q : j); };
+        auto job_of = [&](int j) { return NQ == 2 ? 2 * (done + j) + q : done + j; };
         auto qk = [&](int j) {
-          const int buf = job_of(j) & 1, load = load0 + k_unit(j) * SPT;
+          const int buf = job_of(j) & 1, load = (2 * done + k_unit(j)) * SPT;
 #pragma unroll
           for (int h = 0; h < SPT; ++h) {
             if (!ok || !(ok = full_of(load + h))) return;
@@ -339,12 +500,13 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                                (h | kb | k) != 0);
               if (h == SPT - 1) umma_commit(&s_full[buf]);
               umma_commit(&empty[slot]);
+              if (h == SPT - 1 && j + 1 == take) umma_commit(&q_empty);
             }
             __syncwarp();
           }
         };
         auto pv = [&](int j) {
-          const int job = job_of(j), buf = job & 1, load = load0 + v_unit(j) * SPT;
+          const int job = job_of(j), buf = job & 1, load = (2 * done + v_unit(j, take)) * SPT;
           // V is there before the weights are; these come in two halves of the keys
 #pragma unroll
           for (int h = 0; h < SPT; ++h)
@@ -364,219 +526,396 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
               for (int k = 0; k < 4; ++k)  // 16 keys (2048 bytes of V rows) a step
                 umma_f16_ta(to, tp + 8 * k, dv + 128 * k, id_o, k == 0 ? more : 1u);
               if (h == 1) umma_commit(&pv_done[buf]);
-              if (h >= 2 - SPT) umma_commit(&empty[slot]);
+              // (the slot of a piece's last V is given back by the warps that stage its output in it)
+              if (h >= 2 - SPT && (h == 0 || j + 1 < take)) umma_commit(&empty[slot]);
             }
             __syncwarp();
           }
         };
-        constexpr int kAhead = NQ == 2 ? 1 : 2;  // tiles of logits before the first weights
+        for (;;) {
+          ok = ok && bar_wait(&q_full, pieces & 1, a.err, tc::ERR_TIMEOUT_MMA);
+          if (!ok) break;
+          take = s_piece[pieces & 1].take;
+          ++pieces;
+          if (take == 0) {
+            if (lane == 0) mbar_arrive(&q_empty);
+            break;
+          }
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-          if (j < n) qk(j);
-        for (int j = 0; j < n && ok; ++j) {
-          pv(j);
-          if (j + kAhead < n) qk(j + kAhead);
+          for (int j = 0; j < kAhead; ++j)
+            if (j < take) qk(j);
+          for (int j = 0; j < take && ok; ++j) {
+            pv(j);
+            if (j + kAhead < take) qk(j + kAhead);
+          }
+          done += take;
         }
         // every issued MMA completes before TMEM is released
         if (elect_one()) umma_commit(&drain);
         __syncwarp();
         bar_wait(&drain, pass, a.err, tc::ERR_TIMEOUT_MMA, false);
       }
-      __syncwarp();
+      if (!block_any<C::THREADS>(false)) break;
     }
-    if (!block_any<C::THREADS>(false)) break;
-   }
   } else {
-   if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-   for (int pass = 0; pass < 2; ++pass) {
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ---- softmax and output: one thread per query row ----
+    const int wg = (warp - 4) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)(q4 * 32) << 16);
+    const uint32_t tO = tl + C::O_COL + wg * HD;
+    int done = 0, pieces = 0;
+    bool ok = true;
+    if (NQ == 2 && wg == 1) bar_arrive<256>(2);  // the first turn is warpgroup 0's
+    for (int pass = 0; pass < 2; ++pass) {
+      PromptMeta meta{0, 0, 0, 0};
       bool again = false;
-      const int load0 = pass * 2 * n * SPT, job0 = pass * NQ * n;
-      // ---- softmax and output: one thread per query row ----
-      const int wg = (warp - 4) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
-      const uint32_t tl = tmem + ((uint32_t)(q4 * 32) << 16);
-      const uint32_t tO = tl + C::O_COL + wg * HD;
-      const int i = p.t0 + wg * tok + r / group;     // the row's query
-      const bool row = r < tok * group && i < p.lq;
-      const int mine = row ? visible(i, p.lq, p.lk, p.prefix) : 0;
-      // keys below this need no mask in this warpgroup's rows
-      const int clear = p.t0 + wg * tok < p.lq ? visible(p.t0 + wg * tok, p.lq, p.lk, p.prefix) : 0;
-      float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int j = 0; j < n; ++j) {
-        const int job = job0 + (NQ == 2 ? 2 * j + wg : j), buf = job & 1;
-        if (ok) ok = bar_wait(&s_full[buf], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
-        ok = __all_sync(~0u, ok);
-        if (ok) {
-          tc_fence_after();
-          float s[128];
+      for (;;) {
+        ok = ok && bar_wait(&q_full, pieces & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        // one failure is everybody's: the warps meet at barriers below
+        ok = softmax_all<NQ>(ok);
+        if (!ok) break;
+        const PromptPiece& pc = s_piece[pieces & 1];
+        ++pieces;
+        const int take = pc.take;
+        if ((tid & 127) == 0) mbar_arrive(&q_empty);
+        if (take == 0) break;
+        const int tq = pc.first + wg * tok;            // the first query of these rows
+        const int i = tq + r / group;                  // the row's
+        const bool row = r < tok * group && i < pc.lq;
+        const int mine = row ? visible(i, pc.lq, pc.lk, pc.prefix) : 0;
+        // keys below these need no mask in this warpgroup's rows
+        const int clear = tq < pc.lq ? visible(tq, pc.lq, pc.lk, pc.prefix) : 0;
+        float m = -INFINITY, l = 0.f;
+        for (int t = 0; t < take; ++t) {
+          const int job = NQ == 2 ? 2 * (done + t) + wg : done + t, buf = job & 1;
+          const int key0 = pc.key0 + t * kKeys;
+          if (ok) ok = bar_wait(&s_full[buf], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+          ok = __all_sync(~0u, ok);
+          if (ok) {
+            tc_fence_after();
+            float s[128], c = a.c;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            tmem_ld32_async(tl + buf * kKeys + 32 * q, reinterpret_cast<uint32_t*>(s) + 32 * q);
-          tmem_wait_ld();
-          float c = a.c;
-          if (c <= 0.f) {  // the largest logit is not the largest product: scale first
+            for (int q = 0; q < 4; ++q)
+              tmem_ld32_async(tl + buf * kKeys + 32 * q, reinterpret_cast<uint32_t*>(s) + 32 * q);
+            tmem_wait_ld();
+            if (c <= 0.f) {  // the largest logit is not the largest product: scale first
 #pragma unroll
-            for (int u = 0; u < 128; ++u) s[u] *= c;
-            c = 1.f;
-          }
-          if ((j + 1) * kKeys > clear) {
-            const int lim = mine - j * kKeys;
-#pragma unroll
-            for (int u = 0; u < 128; ++u) s[u] = u < lim ? s[u] : -INFINITY;
-          }
-          const float top = max128(s) * c;
-          if (j == 0) {
-            m = top;
-          } else if (__any_sync(~0u, top > m + kPromptGrow)) {
-            // the sums so far are complete once the P·V before has finished
-            const int prev = NQ == 2 ? job - 2 : job - 1;
-            ok = bar_wait(&pv_done[prev & 1], (prev >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
-            ok = __all_sync(~0u, ok);
-            if (ok) {
-              float al = 1.f;
-              if (top > m + kPromptGrow) {
-                al = m == -INFINITY ? 0.f : exp2_fast(m - top);
-                m = top;
-                l *= al;
-              }
-              tc_fence_after();
-#pragma unroll 1
-              for (int d = 0; d < HD; d += 32) {
-                uint32_t o[32];
-                tmem_ld32(tO + d, o);
-#pragma unroll
-                for (int u = 0; u < 32; ++u)
-                  o[u] = __float_as_uint(__uint_as_float(o[u]) * al);
-                tmem_st32(tO + d, o);
-              }
+              for (int u = 0; u < 128; ++u) s[u] *= c;
+              c = 1.f;
             }
-          }
-          const float ref = m == -INFINITY ? 0.f : m;
-          const uint64_t c2 = pack2(c, c), r2 = pack2(-ref, -ref);
-          uint64_t sum0 = 0, sum1 = 0;  // two zeros each
+            if (key0 + kKeys > clear) {
+              const int lim = mine - key0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[16];
-#pragma unroll
-            for (int u = 0; u < 16; ++u) {
-              const int at = 32 * q + 2 * u;
-              uint64_t x = fma2(pack2(s[at], s[at + 1]), c2, r2);
-              const float2 f = unpack2(x);
-              x = pack2(exp2_fast(f.x), exp2_fast(f.y));
-              if (u & 1) sum1 = add2(sum1, x);
-              else sum0 = add2(sum0, x);
-              // weights in the type of V, as a 16-bit product asks; their sum is of the fp32 ones
-              const float2 e = unpack2(x);
-              w[u] = Tr<T>::pack(e.x, e.y);
+              for (int u = 0; u < 128; ++u) s[u] = u < lim ? s[u] : -INFINITY;
             }
-            tmem_st16(tl + buf * kKeys + 16 * q, w);
-            if (q == 1) {  // the first 64 weights may go
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (pass == 0 && lane == 0) mbar_arrive(&p_full[buf][0]);
-            }
-          }
-          const float2 sums = unpack2(add2(sum0, sum1));
-          l += sums.x + sums.y;
-          tmem_wait_st();
-          tc_fence_before();
-        }
-        if (pass == 1 && (j + 1) * kKeys > fewest) {
-          // V rows of this tile, in halves for two warpgroups: values that are no numbers become
-          // zero; s_bad keeps the first key of the request that lost one
-          const int load = load0 + v_unit(j) * SPT;
-#pragma unroll
-          for (int h = 0; h < SPT; ++h) {
-            const int s = (load + h) % SLOTS;
-            if (ok) ok = bar_wait(&full[s], ((load + h) / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_EPI);
-            ok = __all_sync(~0u, ok);
-            if (!ok) break;
-            for (int v = tid - 128; v < C::SLOT / 16; v += NQ * 128) {
-              const int key = j * kKeys + h * C::VKEYS + (v / 8) % C::VKEYS;
-              uint4* at = reinterpret_cast<uint4*>(base + s * C::SLOT) + v;
-              uint4 x = *at;
-              T* e = reinterpret_cast<T*>(&x);
-              bool hit = false;
-#pragma unroll
-              for (int u = 0; u < 8; ++u)
-                if (!isfinite(Tr<T>::f(e[u]))) {
-                  e[u] = Tr<T>::t(0.f);
-                  hit = true;
+            const float top = max128(s) * c;
+            if (t == 0) {
+              m = top;
+            } else if (__any_sync(~0u, top > m + kPromptGrow)) {
+              // the sums so far are complete once the P·V before has finished
+              const int prev = NQ == 2 ? job - 2 : job - 1;
+              ok = bar_wait(&pv_done[prev & 1], (prev >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+              ok = __all_sync(~0u, ok);
+              if (ok) {
+                float al = 1.f;
+                if (top > m + kPromptGrow) {
+                  al = m == -INFINITY ? 0.f : exp2_fast(m - top);
+                  m = top;
+                  l *= al;
                 }
-              if (hit) {
-                *at = x;
-                if (key < p.lk) atomicMin(&s_bad, key);
+                tc_fence_after();
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 32) {
+                  uint32_t o[32];
+                  tmem_ld32(tO + d, o);
+#pragma unroll
+                  for (int u = 0; u < 32; ++u)
+                    o[u] = __float_as_uint(__uint_as_float(o[u]) * al);
+                  tmem_st32(tO + d, o);
+                }
               }
             }
+            // The exponentials of the two warpgroups take turns: at the same time they would hold
+            // each other up, and then both leave the tensor cores without work.
+            if constexpr (NQ == 2) bar_sync<256>(2 + wg);
+            const float ref = m == -INFINITY ? 0.f : m;
+            const uint64_t c2 = pack2(c, c), r2 = pack2(-ref, -ref);
+            uint64_t sum0 = 0, sum1 = 0;  // two zeros each
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t pw[16];
+#pragma unroll
+              for (int u = 0; u < 16; ++u) {
+                const float2 f = unpack2(fma2(pack2(s[32 * q + 2 * u], s[32 * q + 2 * u + 1]), c2, r2));
+                const float e0 = exp2_fast(f.x), e1 = exp2_fast(f.y);
+                if (u & 1) sum1 = add2(sum1, pack2(e0, e1));
+                else sum0 = add2(sum0, pack2(e0, e1));
+                // weights in the type of V, as a 16-bit product asks; their sum is of the fp32 ones
+                pw[u] = Tr<T>::pack(e0, e1);
+              }
+              tmem_st16(tl + buf * kKeys + 16 * q, pw);
+              if (q == 1) {  // the first 64 weights may go
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (pass == 0 && lane == 0) mbar_arrive(&p_full[buf][0]);
+              }
+            }
+            const float2 sums = unpack2(add2(sum0, sum1));
+            l += sums.x + sums.y;
+            tmem_wait_st();
+            tc_fence_before();
+            if constexpr (NQ == 2) bar_arrive<256>(3 - wg);
+          } else if constexpr (NQ == 2) {
+            bar_sync<256>(2 + wg);
+            bar_arrive<256>(3 - wg);
           }
-          fence_async_smem();
-          named_sync<1, NQ * 128>();
+          if (pass == 1 && key0 + kKeys > pc.fewest) {
+            // V rows of this tile, by all softmax warps: values that are no numbers become zero;
+            // s_bad keeps the first key of the request that lost one
+            const int load = (2 * done + v_unit(t, take)) * SPT;
+#pragma unroll 1
+            for (int h = 0; h < SPT; ++h) {
+              const int sl = (load + h) % SLOTS;
+              if (ok) ok = bar_wait(&full[sl], ((load + h) / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+              ok = __all_sync(~0u, ok);
+              if (!ok) break;
+#pragma unroll 1
+              for (int v = tid - 128; v < C::SLOT / 16; v += NQ * 128) {
+                const int key = key0 + h * C::VKEYS + (v / 8) % C::VKEYS;
+                uint4* at = reinterpret_cast<uint4*>(base + sl * C::SLOT) + v;
+                uint4 x4 = *at;
+                T* e = reinterpret_cast<T*>(&x4);
+                bool hit = false;
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                  if (!isfinite(Tr<T>::f(e[u]))) {
+                    e[u] = Tr<T>::t(0.f);
+                    hit = true;
+                  }
+                if (hit) {
+                  *at = x4;
+                  if (key < pc.lk) atomicMin(&s_bad, key);
+                }
+              }
+            }
+            fence_async_smem();
+            named_sync<1, NQ * 128>();
+          }
+          __syncwarp();
+          if (ok && lane == 0) {
+            if (pass == 1) mbar_arrive(&p_full[buf][0]);  // only now is V what it should be
+            mbar_arrive(&p_full[buf][1]);
+          }
         }
-        __syncwarp();
-        if (ok && lane == 0) {
-          if (pass == 1) mbar_arrive(&p_full[buf][0]);  // only now is V what it should be
-          mbar_arrive(&p_full[buf][1]);
-        }
-      }
-      if (n > 0) {
-        const int last = job0 + (NQ == 2 ? 2 * (n - 1) + wg : n - 1);
+        const int vslot = ((2 * done + v_unit(take - 1, take)) * SPT + SPT - 1) % SLOTS;
+        const int last = NQ == 2 ? 2 * (done + take - 1) + wg : done + take - 1;
+        done += take;
+        const bool whole = pc.slot < 0;
+        const int64_t row_at = (int64_t)(pc.q0 + i) * a.o_tok +
+                               (int64_t)(pc.kv * group + r % group) * a.o_head;
         if (ok) ok = bar_wait(&pv_done[last & 1], (last >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
         ok = __all_sync(~0u, ok);
         tc_fence_after();
-      }
-      // ---- o = O / l ----
-      T* out = reinterpret_cast<T*>(a.out) + (int64_t)(p.q0 + i) * a.o_tok +
-               (int64_t)(kv * group + r % group) * a.o_head;
-      const float inv = 1.f / l;
-      bool odd = false, all = true;  // some, and every, element that is no number
+        int bad = 0x7fffffff;
+        if (pass == 1) {
+          named_sync<1, NQ * 128>();  // s_bad is final for this piece
+          bad = s_bad;
+          named_sync<1, NQ * 128>();
+          if (tid == 128) s_bad = 0x7fffffff;
+          named_sync<1, NQ * 128>();
+        }
+        // o = O / l, or O as it is for the joining kernel. A row that sees no key is zero, and one of
+        // a kernel that gave up waiting NaN.
+        const float inv = !ok ? NAN : whole ? 1.f / l : 1.f;
+        const uint64_t inv2 = pack2(inv, inv);
+        uint64_t nan2[2] = {0, 0};  // sums of 0·o: NaN once an element is no number
+        // Rows leave through the slot of the piece's last V: a lane has a row, and storing straight
+        // from it every instruction would touch 32 lines of global memory. The loops stay rolled:
+        // code that runs once a piece comes from far away.
+        constexpr int CH = C::STAGE / 16;  // 16-byte chunks of a staged row
+        uint8_t* stage = base + vslot * C::SLOT + (warp - 4) * 32 * C::STAGE;
+        const uint32_t keep = mine > 0 ? ~0u : 0u;
+        constexpr int COLS = C::STAGE / 2;  // dimensions of a staged row
+        if (whole) {
+          // the rows whose chunk this lane stores, 32 / CH at a time
+          T* to[CH];
+#pragma unroll
+          for (int k = 0; k < CH; ++k) {
+            const int rr = k * (32 / CH) + lane / CH;
+            const int64_t at = __shfl_sync(~0u, row ? row_at : (int64_t)-1, rr);
+            to[k] = at < 0 ? nullptr : reinterpret_cast<T*>(a.out) + at + lane % CH * 8;
+          }
 #pragma unroll 1
-      for (int d = 0; d < HD; d += 32) {
-        uint32_t o[32];
-        if (n > 0 && ok) tmem_ld32(tO + d, o);
-        uint4 pk[4];
-        uint32_t* pw = reinterpret_cast<uint32_t*>(pk);
+          for (int d = 0; d < HD; d += COLS) {
+            uint32_t o[32];
+            tmem_ld32(tO + d, o);
 #pragma unroll
-        for (int u = 0; u < 16; ++u) {
-          float x = __uint_as_float(o[2 * u]) * inv, y = __uint_as_float(o[2 * u + 1]) * inv;
-          if (mine == 0) x = y = 0.f;
-          else if (!ok) x = y = NAN;
-          const bool fx = isfinite(x), fy = isfinite(y);
-          odd |= !fx || !fy;
-          all &= !fx && !fy;
-          pw[u] = Tr<T>::pack(x, y);
-        }
-        if (row)
+            for (int u = 0; u < CH; ++u) {
+              uint32_t pw[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) reinterpret_cast<uint4*>(out + d)[u] = pk[u];
-      }
-      tc_fence_before();
-      again = row && odd && ok;
-      if (pass == 1) {
-        named_sync<1, NQ * 128>();  // s_bad is final, and so is the other warpgroup's tile
-        // rows that do see a value that was taken out, unless they are NaN throughout as it is
-        unsigned redo = __ballot_sync(~0u, row && ok && mine > s_bad && !all);
-        while (redo) {
-          const int src = __ffs(redo) - 1;
-          redo &= redo - 1;
-          const int rr = q4 * 32 + src, ii = p.t0 + wg * tok + rr / group;
-          const int64_t h = kv * group + rr % group;
-          const PromptKV<T> src_kv{
-              reinterpret_cast<const T*>(a.k) + p.k0 * a.k_tok + kv * a.k_head,
-              reinterpret_cast<const T*>(a.v) + p.k0 * a.v_tok + kv * a.v_head, a.k_tok, a.v_tok};
-          attend_row(reinterpret_cast<const T*>(a.q) + (p.q0 + ii) * a.q_tok + h * a.q_head, HD,
-                     visible(ii, p.lq, p.lk, p.prefix), a.c, src_kv,
-                     reinterpret_cast<T*>(a.out) + (p.q0 + ii) * a.o_tok + h * a.o_head);
+              for (int e = 0; e < 4; ++e) {
+                const uint64_t y = mul2(pack2(__uint_as_float(o[8 * u + 2 * e]),
+                                              __uint_as_float(o[8 * u + 2 * e + 1])), inv2);
+                nan2[e & 1] = fma2(y, 0, nan2[e & 1]);
+                const float2 f = unpack2(y);
+                pw[e] = Tr<T>::pack(f.x, f.y) & keep;
+              }
+              *reinterpret_cast<uint4*>(stage + lane * C::STAGE + (u ^ (lane & (CH - 1))) * 16) =
+                  make_uint4(pw[0], pw[1], pw[2], pw[3]);
+            }
+            __syncwarp();
+            uint4 v[CH];
+#pragma unroll
+            for (int k = 0; k < CH; ++k) {
+              const int rr = k * (32 / CH) + lane / CH;
+              v[k] = *reinterpret_cast<const uint4*>(stage + rr * C::STAGE +
+                                                     ((lane % CH) ^ (rr & (CH - 1))) * 16);
+            }
+#pragma unroll
+            for (int k = 0; k < CH; ++k)
+              if (to[k]) *reinterpret_cast<uint4*>(to[k] + d) = v[k];
+            __syncwarp();
+          }
+        } else {
+          float* part = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + pc.slot) * C::PARTIAL +
+                        wg * C::PART_TILE;
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 32) {
+            uint32_t o[32];
+            tmem_ld32(tO + d, o);
+#pragma unroll
+            for (int u = 0; u < 32; u += 4) {
+              const uint64_t y0 = mul2(pack2(__uint_as_float(o[u]), __uint_as_float(o[u + 1])), inv2);
+              const uint64_t y1 =
+                  mul2(pack2(__uint_as_float(o[u + 2]), __uint_as_float(o[u + 3])), inv2);
+              nan2[0] = fma2(y0, 0, nan2[0]);
+              nan2[1] = fma2(y1, 0, nan2[1]);
+              const float2 f0 = unpack2(y0), f1 = unpack2(y1);
+              *reinterpret_cast<float4*>(part + ((size_t)(d + u) / 4 * 128 + r) * 4) =
+                  make_float4(f0.x, f0.y, f1.x, f1.y);
+            }
+          }
+        }
+        fence_async_smem();
+        bar_sync<128>(4 + wg);
+        if (ok && (tid & 127) == 0) mbar_arrive(&empty[vslot]);
+        const float2 nan = unpack2(add2(nan2[0], nan2[1]));
+        const bool odd = row && mine > 0 && ok && !(nan.x + nan.y == 0.f);
+        again |= odd;
+        // rows that do see a value that was taken out, unless nothing in them is a number anyway
+        bool fix = false;
+        if (pass == 1 && __any_sync(~0u, mine > bad)) {
+          bool all = true;
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 32) {
+            uint32_t o[32];
+            tmem_ld32(tO + d, o);
+#pragma unroll
+            for (int u = 0; u < 32; ++u) all &= !isfinite(__uint_as_float(o[u]));
+          }
+          fix = row && ok && mine > bad && !all;
+        }
+        tc_fence_before();
+        if (!whole) {
+          float* ml = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + pc.slot) * C::PARTIAL +
+                      wg * C::PART_TILE + 128 * HD;
+          ml[r] = m;
+          ml[128 + r] = fix ? -1.f : l;  // no sum is negative: a sign for the joining kernel
+          if (pc.count > 0) meta = PromptMeta{pc.request, pc.tile, pc.kv, pc.count};
+        } else if (pass == 1) {
+          unsigned redo = __ballot_sync(~0u, fix);
+          while (redo) {
+            const int rr = q4 * 32 + __ffs(redo) - 1, ii = tq + rr / group;
+            redo &= redo - 1;
+            const int64_t hh = pc.kv * group + rr % group;
+            const PromptKV<T> src{
+                reinterpret_cast<const T*>(a.k) + pc.k0 * a.k_tok + pc.kv * a.k_head,
+                reinterpret_cast<const T*>(a.v) + pc.k0 * a.v_tok + pc.kv * a.v_head, a.k_tok, a.v_tok};
+            attend_row(reinterpret_cast<const T*>(a.q) + (pc.q0 + ii) * a.q_tok + hh * a.q_head, HD,
+                       visible(ii, pc.lq, pc.lk, pc.prefix), a.c, src,
+                       reinterpret_cast<T*>(a.out) + (pc.q0 + ii) * a.o_tok + hh * a.o_head);
+          }
         }
       }
+      if (tid == 128) reinterpret_cast<PromptMeta*>(a.ws)[cta] = meta;
       if (!block_any<C::THREADS>(again)) break;
-   }
+    }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// Joins the partials of the tile that begins in CTA blockIdx.x and ends in another, in the order of
+// the CTAs: one block per (CTA, tile of rows, 32 dimensions), one thread per row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a, int tok, int ctas) {
+  using C = PromptCfg<HD>;
+  pdl_wait();
+  const int cta = blockIdx.x, wg = blockIdx.y / (HD / 32), d0 = blockIdx.y % (HD / 32) * 32;
+  const PromptMeta meta = reinterpret_cast<const PromptMeta*>(a.ws)[cta];
+  if (meta.count == 0) return;
+  const int r = threadIdx.x, group = a.heads / a.kv_heads;
+  PromptSeq seq;
+  seq.load(a, meta.request);
+  const int tq = meta.tile * C::NQ * tok + wg * tok, i = tq + r / group;
+  const bool row = r < tok * group && i < seq.lq;
+  const float* first = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + 1) * C::PARTIAL +
+                       wg * C::PART_TILE;
+  float M = -INFINITY, l = 0.f, o[32];
+  bool fix = false;
+#pragma unroll
+  for (int u = 0; u < 32; ++u) o[u] = 0.f;
+  for (int p = 0; p < meta.count; ++p) {
+    // partial p: slot 1 of the first CTA, slot 0 of those behind it
+    const float* part = first + (p == 0 ? 0 : ((size_t)p * 2 - 1) * C::PARTIAL);
+    const float pm = part[128 * HD + r], pl = part[128 * HD + 128 + r];
+    float4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      v[u] = *reinterpret_cast<const float4*>(part + ((size_t)(d0 / 4 + u) * 128 + r) * 4);
+    fix |= pl < 0.f;
+    const float top = fmaxf(M, pm), ref = top == -INFINITY ? 0.f : top;
+    const float old = exp2f(M - ref), f = exp2f(pm - ref);
+    M = top;
+    l = l * old + f * pl;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      o[4 * u] = o[4 * u] * old + f * v[u].x;
+      o[4 * u + 1] = o[4 * u + 1] * old + f * v[u].y;
+      o[4 * u + 2] = o[4 * u + 2] * old + f * v[u].z;
+      o[4 * u + 3] = o[4 * u + 3] * old + f * v[u].w;
+    }
+  }
+  const int64_t h = meta.kv * group + r % group;
+  if (row && !fix) {
+    const float inv = 1.f / l;
+    const uint32_t keep = seq.sees(i) > 0 ? ~0u : 0u;  // a row that sees no key is zero
+    T* out = reinterpret_cast<T*>(a.out) + (int64_t)(seq.q0 + i) * a.o_tok + h * a.o_head + d0;
+#pragma unroll
+    for (int u = 0; u < 32; u += 8) {
+      uint4 pk;
+      uint32_t* pw = reinterpret_cast<uint32_t*>(&pk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pw[e] = Tr<T>::pack(o[u + 2 * e] * inv, o[u + 2 * e + 1] * inv) & keep;
+      *reinterpret_cast<uint4*>(out + u) = pk;
+    }
+  }
+  unsigned redo = d0 == 0 ? __ballot_sync(~0u, row && fix) : 0u;
+  while (redo) {
+    const int rr = (r & ~31) + __ffs(redo) - 1, ii = tq + rr / group;
+    redo &= redo - 1;
+    const int64_t hh = meta.kv * group + rr % group;
+    const PromptKV<T> src{reinterpret_cast<const T*>(a.k) + seq.k0 * a.k_tok + meta.kv * a.k_head,
+                          reinterpret_cast<const T*>(a.v) + seq.k0 * a.v_tok + meta.kv * a.v_head,
+                          a.k_tok, a.v_tok};
+    attend_row(reinterpret_cast<const T*>(a.q) + (seq.q0 + ii) * a.q_tok + hh * a.q_head, HD,
+               seq.sees(ii), a.c, src,
+               reinterpret_cast<T*>(a.out) + (seq.q0 + ii) * a.o_tok + hh * a.o_head);
   }
 }
 

@@ -150,6 +150,25 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// `total` pieces of work, numbered in one row, in contiguous shares of `each` or, the first `extra`
+// ones, one more; no share is empty, so fewer pieces than CTAs leave the last CTAs without one.
+template <typename I>
+struct Shares {
+  I each, extra;
+  __device__ __forceinline__ Shares(I total, int ctas) {
+    const I some = max((I)1, min(total, (I)ctas));
+    each = total / some;
+    extra = total - each * some;
+  }
+  __device__ __forceinline__ I begin(int cta, I total) const {
+    return min(total, cta * each + min((I)cta, extra));
+  }
+  __device__ __forceinline__ int owner(I at) const {
+    const I wide = extra * (each + 1);
+    return (int)(at < wide ? at / (each + 1) : extra + (at - wide) / each);
+  }
+};
+
 // ---- two fp32 at a time: the packed forms issue once for both ----
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
   uint64_t r;
@@ -169,6 +188,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -201,6 +225,16 @@ __device__ __forceinline__ bool block_any(bool v) {
       : "r"((uint32_t)v), "n"(N)
       : "memory");
   return r != 0;
+}
+
+// barrier `id` of N threads, some of which only say that they have come
+template <int N>
+__device__ __forceinline__ void bar_sync(int id) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bar_arrive(int id) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory");
 }
 
 template <int ID, int N>

@@ -49,13 +49,13 @@ EXPORTED = (
     "pi0_vision_launch_count", "pi0_vision_device_error", "pi0_vision_profile_enable",
     "pi0_vision_profile_read",
     "pi0_build_slots", "pi0_write_kv", "pi0_attention_prompt", "pi0_attention_paged",
-    "pi0_attention_paged_workspace",
+    "pi0_attention_paged_workspace", "pi0_attention_prompt_workspace",
 )
 
 
 # the entry points behind the binding, in the order that it takes them
 PAGED = ("pi0_build_slots", "pi0_write_kv", "pi0_attention_prompt", "pi0_attention_paged",
-         "pi0_attention_paged_workspace")
+         "pi0_attention_prompt_workspace", "pi0_attention_paged_workspace")
 
 
 def _sources():
@@ -245,7 +245,9 @@ def load():
                                      kv8, vp, vp]
         lib.pi0_attention_prompt.argtypes = [i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, i32,
                                              i32, i32, i32, i32, i32, vp, vp, vp, f32, vp, i64,
-                                             i64, vp, vp]
+                                             i64, vp, i64, vp, vp]
+        lib.pi0_attention_prompt_workspace.argtypes = [i32, i32, i32]
+        lib.pi0_attention_prompt_workspace.restype = ctypes.c_int64
         lib.pi0_attention_paged.argtypes = [i32, vp, i64, i64, i32, i32, kv8, vp, i64, i32, vp,
                                             f32, vp, i64, i64, vp, i64, vp, vp]
         lib.pi0_attention_paged_workspace.argtypes = [i32, i32, i32, i32]

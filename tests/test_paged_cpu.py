@@ -57,8 +57,8 @@ def test_c_entry_points_refuse():
 
     def prompt(dtype=1, q=one, heads=8, kv_heads=2, dim=64, cu=one, total=4, out=one, tok=512, batch=1):
         return lib.pi0_attention_prompt(dtype, q, tok, 64, one, 128, 64, one, 128, 64, total, 4, heads,
-                                        kv_heads, dim, batch, cu, one, None, 0.125, out, 512, 64, None,
-                                        None)
+                                        kv_heads, dim, batch, cu, one, None, 0.125, out, 512, 64, None, 0,
+                                        None, None)
 
     assert [prompt(dtype=3), prompt(q=None), prompt(heads=7), prompt(kv_heads=0), prompt(dim=12),
             prompt(dim=264), prompt(cu=None), prompt(total=-1), prompt(out=ctypes.c_void_p(4100)),
