@@ -124,9 +124,9 @@ struct PromptSeq {
   }
 };
 
-// Writing a tile's rows takes about as long as a step, so in the shares a (tile, kv head) counts for
-// one more than its steps.
-constexpr int kTileCost = 1;
+// Writing a tile's rows takes about as long as a step (6000 clocks to 2500 with 256 dimensions, 4000
+// to 3900 below), so in the shares a (tile, kv head) counts for more than its steps.
+__host__ __device__ constexpr int tile_cost(int head_dim) { return head_dim == 256 ? 2 : 1; }
 
 // A CTA's steps as pieces, each a run of steps of one (tile, kv head). Every role walks the same.
 struct PromptWalk {
@@ -159,7 +159,7 @@ struct PromptWalk {
     at += take;
     j0 += take;
     if (j0 < n) return;  // the share ends inside the tile
-    at += n + kTileCost - j0;
+    at += n + tile_cost(a.head_dim) - j0;
     j0 = 0;
     if (++kv < a.kv_heads) return;
     kv = 0;
@@ -192,15 +192,15 @@ __device__ __forceinline__ float max128(const float (&s)[128]) {
   return fmaxf(max3(a, s[124], s[125]), max3(max3(b, s[126], s[127]), c, d));
 }
 
-// whether all softmax threads say so: they leave their loops together
+// whether all threads of NQ softmax warpgroups say so: they leave their loops together
 template <int NQ>
-__device__ __forceinline__ bool softmax_all(bool v) {
+__device__ __forceinline__ bool softmax_all(bool v, int id = 1) {
   uint32_t r;
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, %2, p;\n"
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n"
       " selp.u32 %0, 1, 0, q;\n}\n"
       : "=r"(r)
-      : "r"((uint32_t)v), "n"(NQ * 128)
+      : "r"((uint32_t)v), "r"(id), "n"(NQ * 128)
       : "memory");
   return r != 0;
 }
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = base + SLOTS * C::SLOT;
   __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, q_empty, s_full[2],
-      p_full[2][2], pv_done[2], drain;
+      p_full[2][2], pv_done[2], turn[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ int s_tiles[C::THREADS], s_scan[WARPS], s_at[4], s_bad;
   __shared__ int64_t s_steps[WARPS], s_begin, s_total;
@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       mbar_init(&p_full[i][0], 4);
       mbar_init(&p_full[i][1], 4);
       mbar_init(&pv_done[i], 1);
+      mbar_init(&turn[i], 4);
     }
     mbar_init(&drain, NQ);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         nt = tiles_of(++b);
         if (nt > 0) seq.load(a, b);
       }
-      return seq.steps(t++ * span, span) + kTileCost;
+      return seq.steps(t++ * span, span) + tile_cost(HD);
     };
     for (int g = g0; g < g1; ++g) sum += steps_of_next();
     sum *= a.kv_heads;
@@ -565,14 +566,14 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
     const uint32_t tO = tl + C::O_COL + wg * HD;
     int done = 0, pieces = 0;
     bool ok = true;
-    if (NQ == 2 && wg == 1) bar_arrive<256>(2);  // the first turn is warpgroup 0's
+    if (NQ == 2 && wg == 1 && lane == 0) mbar_arrive(&turn[0]);  // warpgroup 0's is the first
     for (int pass = 0; pass < 2; ++pass) {
       PromptMeta meta{0, 0, 0, 0};
       bool again = false;
       for (;;) {
         ok = ok && bar_wait(&q_full, pieces & 1, a.err, tc::ERR_TIMEOUT_EPI);
-        // one failure is everybody's: the warps meet at barriers below
-        ok = softmax_all<NQ>(ok);
+        // in the second pass the warpgroups meet below: there one's failure is the other's
+        ok = pass == 1 ? softmax_all<NQ>(ok) : softmax_all<1>(ok, 2 + wg);
         if (!ok) break;
         const PromptPiece& pc = s_piece[pieces & 1];
         ++pieces;
@@ -637,7 +638,8 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             }
             // The exponentials of the two warpgroups take turns: at the same time they would hold
             // each other up, and then both leave the tensor cores without work.
-            if constexpr (NQ == 2) bar_sync<256>(2 + wg);
+            if constexpr (NQ == 2)
+              ok = bar_wait(&turn[wg], (done + t) & 1, a.err, tc::ERR_TIMEOUT_EPI);
             const float ref = m == -INFINITY ? 0.f : m;
             const uint64_t c2 = pack2(c, c), r2 = pack2(-ref, -ref);
             uint64_t sum0 = 0, sum1 = 0;  // two zeros each
@@ -665,10 +667,8 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             l += sums.x + sums.y;
             tmem_wait_st();
             tc_fence_before();
-            if constexpr (NQ == 2) bar_arrive<256>(3 - wg);
-          } else if constexpr (NQ == 2) {
-            bar_sync<256>(2 + wg);
-            bar_arrive<256>(3 - wg);
+            __syncwarp();
+            if (NQ == 2 && lane == 0) mbar_arrive(&turn[wg ^ 1]);
           }
           if (pass == 1 && key0 + kKeys > pc.fewest) {
             // V rows of this tile, by all softmax warps: values that are no numbers become zero;
@@ -746,10 +746,15 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             const int64_t at = __shfl_sync(~0u, row ? row_at : (int64_t)-1, rr);
             to[k] = at < 0 ? nullptr : reinterpret_cast<T*>(a.out) + at + lane % CH * 8;
           }
+          uint32_t next[32];
+          tmem_ld32_async(tO, next);
 #pragma unroll 1
           for (int d = 0; d < HD; d += COLS) {
             uint32_t o[32];
-            tmem_ld32(tO + d, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int u = 0; u < 32; ++u) o[u] = next[u];
+            if (d + COLS < HD) tmem_ld32_async(tO + d + COLS, next);
 #pragma unroll
             for (int u = 0; u < CH; ++u) {
               uint32_t pw[4];
