@@ -201,7 +201,7 @@ int run_paged(const DecodeArgs& a, int device, int sms, cudaStream_t st) {
   if (cudaGetLastError() != cudaSuccess) return PI0_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, std::min(NH, group));
-  cfg.blockDim = dim3(HD);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -351,66 +351,73 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     __syncwarp();
   } else if (warp == 1) {
     // ---- MMA issuer ----
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc_e4m3(128, N, false, false);
-      constexpr uint32_t id_o = idesc_e4m3(128, N, true, true);
-      const uint32_t ring = smem_u32(base);
-      bool ok = true;
-      int g = 0, piece = 0;  // tiles and pieces so far
-      // tile g of the CTA has its K in load 2g and its V in load 2g + 1
-      auto full_of = [&](int load) {
-        return mbar_wait(&full[load % C::SLOTS], (load / C::SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
-      };
-      auto qk = [&](int i) -> bool {
-        const int slot = (2 * i) % C::SLOTS;
-        if (!full_of(2 * i)) return false;
-        if (i >= 2 && !mbar_wait(&s_free[i & 1], ((i >> 1) - 1) & 1, a.err, tc::ERR_TIMEOUT_MMA))
-          return false;
-        tc_fence_after();
-        const uint32_t d = tmem + C::S_COL + (i & 1) * N;
+    constexpr uint32_t id_s = idesc_e4m3(128, N, false, false);
+    constexpr uint32_t id_o = idesc_e4m3(128, N, true, true);
+    const uint32_t ring = __shfl_sync(~0u, smem_u32(base), 0), tm = __shfl_sync(~0u, tmem, 0);
+    const uint32_t qs = ring + C::SLOTS * C::SLOT, pb = qs + C::Q_BYTES;
+    bool ok = true;
+    int g = 0, piece = 0;  // tiles and pieces so far
+    // tile g of the CTA has its K in load 2g and its V in load 2g + 1
+    auto full_of = [&](int load) {
+      return mbar_wait(&full[load % C::SLOTS], (load / C::SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
+    };
+    auto qk = [&](int i) -> bool {
+      const int slot = (2 * i) % C::SLOTS;
+      if (!full_of(2 * i)) return false;
+      if (i >= 2 && !mbar_wait(&s_free[i & 1], ((i >> 1) - 1) & 1, a.err, tc::ERR_TIMEOUT_MMA))
+        return false;
+      tc_fence_after();
+      const uint64_t dk = sdesc<ROW>(ring + slot * C::SLOT, 8 * ROW, 0);
+      const uint64_t dq = sdesc<ROW>(qs, 8 * ROW, 0);
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < HD / 32; ++k) {
-          const uint32_t off = (k % (ROW / 32)) * 32, blk = k / (ROW / 32);
-          umma_f8(d, sdesc<ROW>(ring + slot * C::SLOT + blk * C::BLOCK + off, 8 * ROW, 0),
-                  sdesc<ROW>(smem_u32(sQ) + blk * (N * ROW) + off, 8 * ROW, 0), id_s, k != 0);
+          constexpr int PER = ROW / 32;  // steps of 32 bytes in a row
+          umma_f8(tm + C::S_COL + (i & 1) * N, dk + (k / PER * C::BLOCK + k % PER * 32) / 16,
+                  dq + (k / PER * (N * ROW) + k % PER * 32) / 16, id_s, k != 0);
         }
         umma_commit(&s_full[i & 1]);
         umma_commit(&empty[slot]);
-        return true;
-      };
-      auto pv = [&](int i, bool first) -> bool {
-        const int slot = (2 * i + 1) % C::SLOTS;
-        if (!mbar_wait(&p_full[i & 1], (i >> 1) & 1, a.err, tc::ERR_TIMEOUT_MMA) ||
-            !full_of(2 * i + 1))
-          return false;
-        tc_fence_after();
+      }
+      __syncwarp();
+      return true;
+    };
+    auto pv = [&](int i, bool first) -> bool {
+      const int slot = (2 * i + 1) % C::SLOTS;
+      if (!full_of(2 * i + 1) ||
+          !mbar_wait(&p_full[i & 1], (i >> 1) & 1, a.err, tc::ERR_TIMEOUT_MMA))
+        return false;
+      tc_fence_after();
+      // 64-wide heads: both halves of M read the same 64 dimensions (lbo 0)
+      const uint64_t dv = sdesc<ROW>(ring + slot * C::SLOT, 8 * ROW, 0);
+      const uint64_t dp = sdesc<N>(pb + (i & 1) * C::P_BYTES, 8 * N, 0);
+      const uint32_t more = !first;
+      if (elect_one()) {
 #pragma unroll
         for (int hb = 0; hb < C::HB; ++hb)
 #pragma unroll
           for (int k = 0; k < kDecTile / 32; ++k)  // 32 keys a step
-            umma_f8(tmem + C::O_COL + hb * N,
-                    // 64-wide heads: both halves of M read the same 64 dimensions (lbo 0)
-                    sdesc<ROW>(ring + slot * C::SLOT + hb * C::BLOCK + k * 32 * ROW, 8 * ROW, 0),
-                    sdesc<N>(smem_u32(sP) + (i & 1) * C::P_BYTES + k * 32 * N, 8 * N, 0), id_o,
-                    !(first && k == 0));
-        umma_commit(&empty[slot]);
+            umma_f8(tm + C::O_COL + hb * N, dv + (hb * C::BLOCK + k * 32 * ROW) / 16,
+                    dp + k * 32 * N / 16, id_o, k == 0 ? more : 1u);
         umma_commit(&pv_done[i & 1]);
-        return true;
-      };
-      while (ok && w.next()) {
-        ok = mbar_wait(&q_full, piece & 1, a.err, tc::ERR_TIMEOUT_MMA) && qk(g);
-        for (int i = 0; i < w.take && ok; ++i, ++g) {
-          if (i + 1 < w.take) ok = qk(g + 1);
-          ok = ok && pv(g, i == 0);
-        }
-        ++piece;
-        w.done();
+        umma_commit(&empty[slot]);
       }
-      // every issued MMA completes before TMEM is released
-      umma_commit(&drain);
-      mbar_wait(&drain, 0, a.err, tc::ERR_TIMEOUT_MMA, false);
+      __syncwarp();
+      return true;
+    };
+    while (ok && w.next()) {
+      ok = mbar_wait(&q_full, piece & 1, a.err, tc::ERR_TIMEOUT_MMA) && qk(g);
+      for (int i = 0; i < w.take && ok; ++i, ++g) {
+        if (i + 1 < w.take) ok = qk(g + 1);
+        ok = ok && pv(g, i == 0);
+      }
+      ++piece;
+      w.done();
     }
+    // every issued MMA completes before TMEM is released
+    if (elect_one()) umma_commit(&drain);
     __syncwarp();
+    mbar_wait(&drain, 0, a.err, tc::ERR_TIMEOUT_MMA, false);
   } else {
     // ---- softmax and output: warps 2-5 ----
     const int q4 = warp & 3, r = q4 * 32 + lane;
@@ -696,20 +703,24 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
 }
 
 // Joins the partials of the unit that begins in CTA blockIdx.x and ends in another: one block per
-// (CTA, head), out = Σ 2^(Mᵢ−M)·oᵢ / (16·Σ 2^(Mᵢ−M)·lᵢ) over the CTAs in order.
+// (CTA, head), out = Σ 2^(Mᵢ−M)·oᵢ / (16·Σ 2^(Mᵢ−M)·lᵢ). A thread takes one dimension of every JS-th
+// eight partials, whose loads are in flight together; the JS sums are joined in order.
+constexpr int kJoinThreads = 512;
+
 template <typename T, int HD, int NH>
-__global__ void __launch_bounds__(HD) paged_join_kernel(DecodeArgs a, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(DecodeArgs a, int ctas) {
   using C = DecCfg<HD, NH>;
+  constexpr int JS = kJoinThreads / HD;
+  __shared__ float s_o[JS][HD], s_m[JS], s_l[JS];
   pdl_wait();
-  const int cta = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
+  const int cta = blockIdx.x, h = blockIdx.y, d = threadIdx.x % HD, js = threadIdx.x / HD;
   const DecMeta meta = reinterpret_cast<const DecMeta*>(a.ws)[cta];
   if (h >= meta.heads || meta.count == 0) return;
   const float* first = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + 1) * C::PARTIAL;
   // partial i: slot 1 of the first CTA, slot 0 of those behind it
   auto part = [&](int i) { return first + (i == 0 ? 0 : ((size_t)i * 2 - 1) * C::PARTIAL); };
-  // eight partials at a time, so that their loads are in flight together
   float M = -INFINITY, o = 0.f, l = 0.f;
-  for (int i0 = 0; i0 < meta.count; i0 += 8) {
+  for (int i0 = js * 8; i0 < meta.count; i0 += JS * 8) {
     float pm[8], pl[8], po[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -733,8 +744,28 @@ __global__ void __launch_bounds__(HD) paged_join_kernel(DecodeArgs a, int ctas) 
       l = fmaf(f, pl[i], l);
     }
   }
-  reinterpret_cast<T*>(a.out)[meta.batch * a.o_tok + (meta.head + h) * a.o_head + d] =
-      Tr<T>::t(o / (16.f * l));
+  if (meta.count > 8) {  // uniform: a block has one unit
+    s_o[js][d] = o;
+    if (d == 0) {
+      s_m[js] = M;
+      s_l[js] = l;
+    }
+    __syncthreads();
+    float top = s_m[0];
+#pragma unroll
+    for (int j = 1; j < JS; ++j) top = fmaxf(top, s_m[j]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    o = l = 0.f;
+#pragma unroll
+    for (int j = 0; j < JS; ++j) {
+      const float f = exp2f(s_m[j] - ref);
+      o = fmaf(f, s_o[j][d], o);
+      l = fmaf(f, s_l[j], l);
+    }
+  }
+  if (js == 0)
+    reinterpret_cast<T*>(a.out)[meta.batch * a.o_tok + (meta.head + h) * a.o_head + d] =
+        Tr<T>::t(o / (16.f * l));
 }
 
 }  // namespace paged
