@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 #include "pi0b200.h"
 #include "paged_slots.cuh"
@@ -170,8 +171,12 @@ bool paged_tc(int head_dim, int page_size, int64_t planes) {
          (page_size % 128 == 0 || (page_size % 8 == 0 && 128 % page_size == 0)) && planes <= INT_MAX;
 }
 
-// heads of a unit's columns: 8 cover most groups; wider groups go 16 at a time
-int paged_heads(int heads, int kv_heads) { return heads / kv_heads <= 8 ? 8 : 16; }
+// Heads of a unit's columns: the softmax does its work for all of them, so groups of up to 4 and up
+// to 8 have their own; wider groups go 16 at a time.
+int paged_heads(int heads, int kv_heads) {
+  const int group = heads / kv_heads;
+  return group <= 4 ? 4 : group <= 8 ? 8 : 16;
+}
 
 template <int HD, int NH>
 int64_t paged_ws(int sms) {
@@ -214,11 +219,17 @@ int run_paged(const DecodeArgs& a, int device, int sms, cudaStream_t st) {
 
 template <typename T>
 int run_paged_any(const DecodeArgs& a, int device, int sms, cudaStream_t st) {
-  const bool wide = paged_heads(a.heads, a.cache.kv_heads) == 16;
+  const int nh = paged_heads(a.heads, a.cache.kv_heads);
+  auto run = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    return nh == 4   ? run_paged<T, HD, 4>(a, device, sms, st)
+           : nh == 8 ? run_paged<T, HD, 8>(a, device, sms, st)
+                     : run_paged<T, HD, 16>(a, device, sms, st);
+  };
   switch (a.cache.head_dim) {
-    case 64: return wide ? run_paged<T, 64, 16>(a, device, sms, st) : run_paged<T, 64, 8>(a, device, sms, st);
-    case 128: return wide ? run_paged<T, 128, 16>(a, device, sms, st) : run_paged<T, 128, 8>(a, device, sms, st);
-    default: return wide ? run_paged<T, 256, 16>(a, device, sms, st) : run_paged<T, 256, 8>(a, device, sms, st);
+    case 64: return run(std::integral_constant<int, 64>());
+    case 128: return run(std::integral_constant<int, 128>());
+    default: return run(std::integral_constant<int, 256>());
   }
 }
 
@@ -345,11 +356,15 @@ int64_t pi0_attention_paged_workspace(int heads, int kv_heads, int head_dim, int
   int device;
   const int sms = sm_count(&device);
   if (!sms) return -1;
-  const bool wide = paged_heads(heads, kv_heads) == 16;
+  const int nh = paged_heads(heads, kv_heads);
+  auto bytes = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    return nh == 4 ? paged_ws<HD, 4>(sms) : nh == 8 ? paged_ws<HD, 8>(sms) : paged_ws<HD, 16>(sms);
+  };
   switch (head_dim) {
-    case 64: return wide ? paged_ws<64, 16>(sms) : paged_ws<64, 8>(sms);
-    case 128: return wide ? paged_ws<128, 16>(sms) : paged_ws<128, 8>(sms);
-    default: return wide ? paged_ws<256, 16>(sms) : paged_ws<256, 8>(sms);
+    case 64: return bytes(std::integral_constant<int, 64>());
+    case 128: return bytes(std::integral_constant<int, 128>());
+    default: return bytes(std::integral_constant<int, 256>());
   }
 }
 

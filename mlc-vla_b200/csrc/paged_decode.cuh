@@ -116,12 +116,16 @@ struct DecCfg {
   static constexpr int HB = (HD + 127) / 128;       // 128-wide blocks of the head dimension
   static constexpr int SLOT = kDecTile * HD;        // a K or a V tile
   static constexpr int BLOCK = kDecTile * ROW;      // one 128-wide block of it
-  static constexpr int N = 4 * NH;                  // columns: three parts (and one empty) × heads
+  // columns: three parts × heads, then empty ones; COLS of them are read back
+  static constexpr int N = NH < 8 ? 32 : 4 * NH;
+  static constexpr int COLS = 4 * NH;
   static constexpr int Q_BYTES = N * HD;
   static constexpr int P_BYTES = kDecTile * N;
   static constexpr int FIXED = Q_BYTES + 2 * P_BYTES + 1024;
-  static constexpr int OCC = HD < 256 && NH == 8 ? 2 : 1;  // CTAs per SM (16 heads: registers)
-  static constexpr int ROOM = (OCC == 2 ? 110 * 1024 : 225 * 1024) - FIXED;
+  // CTAs per SM: a narrow head's tile loads faster than one softmax warpgroup takes it (16 heads:
+  // no registers for a second)
+  static constexpr int OCC = HD == 256 || NH > 8 ? 1 : HD == 64 && NH == 4 ? 3 : 2;
+  static constexpr int ROOM = (OCC == 1 ? 225 : OCC == 2 ? 110 : 72) * 1024 - FIXED;
   static constexpr int SLOTS = (ROOM / SLOT) & ~1;
   static constexpr int SMEM = SLOTS * SLOT + FIXED;
   static constexpr int S_COL = 0, O_COL = 2 * N;
@@ -422,6 +426,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     // ---- softmax and output: warps 2-5 ----
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t tlane = tmem + ((uint32_t)(q4 * 32) << 16);
+    constexpr int STEP = C::COLS < 32 ? 16 : 32;  // columns read at a time
     bool ok = true;
     int g = 0;
     int x = s_begin;
@@ -509,11 +514,11 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
         if (ok) {
           tc_fence_after();
 #pragma unroll
-          for (int n0 = 0; n0 < N; n0 += 32) {
-            uint32_t raw[32];
-            tmem_ld32(tlane + C::S_COL + buf * N + n0, raw);
+          for (int n0 = 0; n0 < C::COLS; n0 += STEP) {
+            uint32_t raw[STEP];
+            tmem_ld_cols(tlane + C::S_COL + buf * N + n0, raw);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
+            for (int j = 0; j < STEP; ++j) {
               const int p = (n0 + j) / NH, h = (n0 + j) % NH;
               const float f = __uint_as_float(raw[j]);
               if (p == 0) s[h] = f;
@@ -564,13 +569,14 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
           if (ok) {
             tc_fence_after();
 #pragma unroll
-            for (int c0 = 0; c0 < C::HB * N; c0 += 32) {
-              uint32_t o[32];
-              tmem_ld32(tlane + C::O_COL + c0, o);
+            for (int c0 = 0; c0 < C::HB * C::COLS; c0 += STEP) {
+              const uint32_t at = tlane + C::O_COL + c0 / C::COLS * N + c0 % C::COLS;
+              uint32_t o[STEP];
+              tmem_ld_cols(at, o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
+              for (int j = 0; j < STEP; ++j)
                 o[j] = __float_as_uint(__uint_as_float(o[j]) * al[(c0 + j) % NH]);
-              tmem_st32(tlane + C::O_COL + c0, o);
+              tmem_st_cols(at, o);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -598,7 +604,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
         if (ok) {
           uint8_t* p = sP + buf * C::P_BYTES;
 #pragma unroll
-          for (int n0 = 0; n0 < N; n0 += 16) {
+          for (int n0 = 0; n0 < C::COLS; n0 += 16) {
             uint4 q;
             uint32_t* qw = reinterpret_cast<uint32_t*>(&q);
 #pragma unroll
@@ -651,11 +657,11 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
       for (int hb = 0; hb < C::HB; ++hb) {
         float o[NH];
 #pragma unroll
-        for (int n0 = 0; n0 < N; n0 += 32) {
-          uint32_t raw[32];
-          if (ok) tmem_ld32(tlane + C::O_COL + hb * N + n0, raw);
+        for (int n0 = 0; n0 < C::COLS; n0 += STEP) {
+          uint32_t raw[STEP];
+          tmem_ld_cols(tlane + C::O_COL + hb * N + n0, raw);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < STEP; ++j) {
             const int p = (n0 + j) / NH, h = (n0 + j) % NH;
             const float f = ok ? __uint_as_float(raw[j]) : NAN;
             if (p == 0) o[h] = f;

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = base + SLOTS * C::SLOT;
   __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, q_empty, s_full[2],
-      p_full[2][2], pv_done[2], turn[2], drain;
+      p_full[2][2], pv_done[2], o_done, turn[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ int s_tiles[C::THREADS], s_scan[WARPS], s_at[4], s_bad;
   __shared__ int64_t s_steps[WARPS], s_begin, s_total;
@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       mbar_init(&empty[i], NQ);
     }
     mbar_init(&q_full, 1);
+    mbar_init(&o_done, NQ);
     mbar_init(&q_empty, 2 * NQ);  // its QKs are done, and the softmax warps have begun it
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -527,6 +528,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
               for (int k = 0; k < 4; ++k)  // 16 keys (2048 bytes of V rows) a step
                 umma_f16_ta(to, tp + 8 * k, dv + 128 * k, id_o, k == 0 ? more : 1u);
               if (h == 1) umma_commit(&pv_done[buf]);
+              if (h == 1 && j + 1 == take) umma_commit(&o_done);
               // (the slot of a piece's last V is given back by the warps that stage its output in it)
               if (h >= 2 - SPT && (h == 0 || j + 1 < take)) umma_commit(&empty[slot]);
             }
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
     const int wg = (warp - 4) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)(q4 * 32) << 16);
     const uint32_t tO = tl + C::O_COL + wg * HD;
-    int done = 0, pieces = 0;
+    int done = 0, pieces = 0, worked = 0;  // steps; pieces, and those of them that have steps
     bool ok = true;
     if (NQ == 2 && wg == 1 && lane == 0) mbar_arrive(&turn[0]);  // warpgroup 0's is the first
     for (int pass = 0; pass < 2; ++pass) {
@@ -709,12 +711,13 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           }
         }
         const int vslot = ((2 * done + v_unit(take - 1, take)) * SPT + SPT - 1) % SLOTS;
-        const int last = NQ == 2 ? 2 * (done + take - 1) + wg : done + take - 1;
         done += take;
         const bool whole = pc.slot < 0;
         const int64_t row_at = (int64_t)(pc.q0 + i) * a.o_tok +
                                (int64_t)(pc.kv * group + r % group) * a.o_head;
-        if (ok) ok = bar_wait(&pv_done[last & 1], (last >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        // the last P·V of every tile of rows: the slot of the last V is about to be written
+        if (ok) ok = bar_wait(&o_done, worked & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        ++worked;
         ok = __all_sync(~0u, ok);
         tc_fence_after();
         int bad = 0x7fffffff;

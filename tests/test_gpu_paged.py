@@ -306,6 +306,48 @@ def test_prompt_around_tile_edges(n, heads, dim):
     close(out[some], np.array(want), np.array(tol))
 
 
+@pytest.mark.parametrize("new,held,prefix,heads,kv_heads,dim,dtype", [
+    ([4096], [0], None, 16, 4, 128, "bfloat16"), ([3000, 1111], [0, 777], None, 8, 4, 64, "float16"),
+    ([968, 700, 850, 901] * 3, [0] * 12, [768] * 12, 8, 1, 256, "float16"),
+    ([200, 33, 170], [4000, 2500, 3777], None, 16, 4, 128, "float16"),
+    ([1, 1, 1], [5000, 3, 9000], None, 8, 1, 256, "bfloat16"),
+    ([2500, 1], [0, 1], [2500, 1], 5, 1, 128, "float16")])
+def test_prompt_many_tiles(new, held, prefix, heads, kv_heads, dim, dtype):
+    """Enough tiles that a CTA works on several and shares some with others."""
+    from mlc_vla import paged
+
+    q, k, v, cu_q, cu_k, prefix = prompt_case(new, held, prefix, heads, kv_heads, dim, dtype, seed=dim)
+    out = paged.attention_prompt(q, k, v, dev(cu_q), dev(cu_k),
+                                 prefix_lens=None if prefix is None else dev(prefix))
+    paged.check()
+    rng = np.random.default_rng(0)
+    kn, vn = num(k), num(v)
+    for r in range(len(new)):
+        first, n = cu_k[r], cu_k[r + 1] - cu_k[r]
+        some = sorted(set(rng.integers(0, new[r], 24)) | {0, new[r] - 1})
+        for i in some:  # one query with the keys it sees
+            t = cu_q[r] + i
+            sees = min(n, max(i + n - new[r] + 1, 0 if prefix is None else prefix[r]))
+            want, tol = R.attention_prompt(num(q[t:t + 1]), kn[first:first + sees],
+                                           vn[first:first + sees], [0, 1], [0, sees], [0],
+                                           dim ** -0.5, dtype)
+            close(out[t:t + 1], want, tol)
+    # every row, against a batched softmax in 64 bits on the GPU, within the same kind of bound
+    group, worst = heads // kv_heads, 0.0
+    for r in range(len(new)):
+        n, i = cu_k[r + 1] - cu_k[r], torch.arange(new[r], device="cuda")[:, None]
+        j = torch.arange(n, device="cuda")[None]
+        seen = (j <= i + n - new[r]) | (j < (0 if prefix is None else prefix[r]))
+        for h in range(heads):
+            kh, vh = (x[cu_k[r]:cu_k[r + 1], h // group].double() for x in (k, v))
+            s = q[cu_q[r]:cu_q[r + 1], h].double() @ kh.T * dim ** -0.5
+            p = torch.softmax(s.masked_fill(~seen, float("-inf")), -1)
+            o, spread = p @ vh, p @ vh.abs()
+            tol = R.UNIT[dtype] * (o.abs() + 2 * spread) + 1e-3 * spread + 2.0 ** -24
+            worst = max(worst, float(((out[cu_q[r]:cu_q[r + 1], h].double() - o).abs() / tol).max()))
+    assert worst <= 1.0, worst
+
+
 def test_prompt_large_logits_and_scales():
     for scale in (1.0, 0.01, -0.3, 0.0):
         check_prompt(prompt_case([90, 33], [0, 100], None, 4, 1, 128, "float16", seed=5), "float16",
