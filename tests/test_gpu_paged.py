@@ -332,7 +332,7 @@ def test_prompt_many_tiles(new, held, prefix, heads, kv_heads, dim, dtype):
                                            vn[first:first + sees], [0, 1], [0, sees], [0],
                                            dim ** -0.5, dtype)
             close(out[t:t + 1], want, tol)
-    # every row, against a batched softmax in 64 bits on the GPU, within the same kind of bound
+    # every row, against a softmax in 64 bits on the GPU, within the bound of paged_ref._attend
     group, worst = heads // kv_heads, 0.0
     for r in range(len(new)):
         n, i = cu_k[r + 1] - cu_k[r], torch.arange(new[r], device="cuda")[:, None]
@@ -343,7 +343,11 @@ def test_prompt_many_tiles(new, held, prefix, heads, kv_heads, dim, dtype):
             s = q[cu_q[r]:cu_q[r + 1], h].double() @ kh.T * dim ** -0.5
             p = torch.softmax(s.masked_fill(~seen, float("-inf")), -1)
             o, spread = p @ vh, p @ vh.abs()
-            tol = R.UNIT[dtype] * (o.abs() + 2 * spread) + 1e-3 * spread + 2.0 ** -24
+            size = (q[cu_q[r]:cu_q[r + 1], h].double().abs() @ kh.abs().T).amax(1, True) * dim ** -0.5
+            logit = 2 * (dim * 2.0 ** -23 * size + 2.0 ** -21 * s.abs().amax(1, True) + 2.0 ** -20)
+            u = R.UNIT[dtype]
+            tol = (u * o.abs() + (2 * u + logit + n * 2.0 ** -23) * spread
+                   + n * 2.0 ** -25 * vh.abs().max() + 2.0 ** -24)
             worst = max(worst, float(((out[cu_q[r]:cu_q[r + 1], h].double() - o).abs() / tol).max()))
     assert worst <= 1.0, worst
 
