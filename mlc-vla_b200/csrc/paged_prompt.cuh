@@ -95,9 +95,6 @@ struct PromptCfg {
   static constexpr int VKEYS = kKeys / SPT;         // keys of a V slot
   // tensor memory: two tiles of logits, each overlaid by its weights, then the sums
   static constexpr int O_COL = 256;
-  // bytes of a row that a warp stages for output at a time: its 32 rows fit its part of a ring slot
-  static constexpr int STAGE = 64;
-  static_assert(4 * NQ * 32 * STAGE <= SLOT, "staged rows of all warps");
   // a partial: for each tile of rows the sums as [HD / 4][128 rows][4], then M and l of the rows
   static constexpr int PART_TILE = 128 * HD + 256;
   static constexpr int PARTIAL = NQ * PART_TILE;
@@ -217,7 +214,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sQ = base + SLOTS * C::SLOT;
   __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, q_empty, s_full[2],
-      p_full[2][2], pv_done[2], o_done, turn[2], drain;
+      p_full[2][2], pv_done[2], turn[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ int s_tiles[C::THREADS], s_scan[WARPS], s_at[4], s_bad;
   __shared__ int64_t s_steps[WARPS], s_begin, s_total;
@@ -233,7 +230,6 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       mbar_init(&empty[i], NQ);
     }
     mbar_init(&q_full, 1);
-    mbar_init(&o_done, NQ);
     mbar_init(&q_empty, 2 * NQ);  // its QKs are done, and the softmax warps have begun it
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -528,9 +524,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
               for (int k = 0; k < 4; ++k)  // 16 keys (2048 bytes of V rows) a step
                 umma_f16_ta(to, tp + 8 * k, dv + 128 * k, id_o, k == 0 ? more : 1u);
               if (h == 1) umma_commit(&pv_done[buf]);
-              if (h == 1 && j + 1 == take) umma_commit(&o_done);
-              // (the slot of a piece's last V is given back by the warps that stage its output in it)
-              if (h >= 2 - SPT && (h == 0 || j + 1 < take)) umma_commit(&empty[slot]);
+              if (h >= 2 - SPT) umma_commit(&empty[slot]);
             }
             __syncwarp();
           }
@@ -566,7 +560,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
     const int wg = (warp - 4) >> 2, q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)(q4 * 32) << 16);
     const uint32_t tO = tl + C::O_COL + wg * HD;
-    int done = 0, pieces = 0, worked = 0;  // steps; pieces, and those of them that have steps
+    int done = 0, pieces = 0;
     bool ok = true;
     if (NQ == 2 && wg == 1 && lane == 0) mbar_arrive(&turn[0]);  // warpgroup 0's is the first
     for (int pass = 0; pass < 2; ++pass) {
@@ -710,14 +704,12 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             mbar_arrive(&p_full[buf][1]);
           }
         }
-        const int vslot = ((2 * done + v_unit(take - 1, take)) * SPT + SPT - 1) % SLOTS;
+        const int last = NQ == 2 ? 2 * (done + take - 1) + wg : done + take - 1;
         done += take;
         const bool whole = pc.slot < 0;
         const int64_t row_at = (int64_t)(pc.q0 + i) * a.o_tok +
                                (int64_t)(pc.kv * group + r % group) * a.o_head;
-        // the last P·V of every tile of rows: the slot of the last V is about to be written
-        if (ok) ok = bar_wait(&o_done, worked & 1, a.err, tc::ERR_TIMEOUT_EPI);
-        ++worked;
+        if (ok) ok = bar_wait(&pv_done[last & 1], (last >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
         ok = __all_sync(~0u, ok);
         tc_fence_after();
         int bad = 0x7fffffff;
@@ -733,57 +725,54 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         const float inv = !ok ? NAN : whole ? 1.f / l : 1.f;
         const uint64_t inv2 = pack2(inv, inv);
         uint64_t nan2[2] = {0, 0};  // sums of 0·o: NaN once an element is no number
-        // Rows leave through the slot of the piece's last V: a lane has a row, and storing straight
-        // from it every instruction would touch 32 lines of global memory. The loops stay rolled:
-        // code that runs once a piece comes from far away.
-        constexpr int CH = C::STAGE / 16;  // 16-byte chunks of a staged row
-        uint8_t* stage = base + vslot * C::SLOT + (warp - 4) * 32 * C::STAGE;
         const uint32_t keep = mine > 0 ? ~0u : 0u;
-        constexpr int COLS = C::STAGE / 2;  // dimensions of a staged row
         if (whole) {
-          // the rows whose chunk this lane stores, 32 / CH at a time
-          T* to[CH];
+          // A lane has a row, and storing straight from it every instruction would touch 32 lines of
+          // global memory. Four lanes exchange chunks of 16 bytes first: lane 4a + c then has chunk c
+          // of the rows 4a, 4a + 1, 4a + 2, 4a + 3. The loop stays rolled: code that runs once a
+          // piece comes from far away.
+          T* to[4];
 #pragma unroll
-          for (int k = 0; k < CH; ++k) {
-            const int rr = k * (32 / CH) + lane / CH;
-            const int64_t at = __shfl_sync(~0u, row ? row_at : (int64_t)-1, rr);
-            to[k] = at < 0 ? nullptr : reinterpret_cast<T*>(a.out) + at + lane % CH * 8;
+          for (int k = 0; k < 4; ++k) {
+            const int64_t at = __shfl_sync(~0u, row ? row_at : (int64_t)-1, (lane & ~3) + k);
+            to[k] = at < 0 ? nullptr : reinterpret_cast<T*>(a.out) + at + (lane & 3) * 8;
           }
           uint32_t next[32];
           tmem_ld32_async(tO, next);
 #pragma unroll 1
-          for (int d = 0; d < HD; d += COLS) {
-            uint32_t o[32];
+          for (int d = 0; d < HD; d += 32) {
+            uint32_t pw[4][4];  // the row's four chunks
             tmem_wait_ld();
 #pragma unroll
-            for (int u = 0; u < 32; ++u) o[u] = next[u];
-            if (d + COLS < HD) tmem_ld32_async(tO + d + COLS, next);
+            for (int u = 0; u < 16; ++u) {
+              const uint64_t y = mul2(pack2(__uint_as_float(next[2 * u]),
+                                            __uint_as_float(next[2 * u + 1])), inv2);
+              nan2[u & 1] = fma2(y, 0, nan2[u & 1]);
+              const float2 f = unpack2(y);
+              pw[u / 4][u % 4] = Tr<T>::pack(f.x, f.y) & keep;
+            }
+            if (d + 32 < HD) tmem_ld32_async(tO + d + 32, next);
+            // transpose of 4 × 4 chunks in two exchanges: with the lane one away, then two away
 #pragma unroll
-            for (int u = 0; u < CH; ++u) {
-              uint32_t pw[4];
+            for (int st = 1; st <= 2; st *= 2) {
+              const bool up = lane & st;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint64_t y = mul2(pack2(__uint_as_float(o[8 * u + 2 * e]),
-                                              __uint_as_float(o[8 * u + 2 * e + 1])), inv2);
-                nan2[e & 1] = fma2(y, 0, nan2[e & 1]);
-                const float2 f = unpack2(y);
-                pw[e] = Tr<T>::pack(f.x, f.y) & keep;
+              for (int c = 0; c < 4; ++c) {
+                if (c & st) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t give = up ? pw[c][e] : pw[c + st][e];
+                  const uint32_t got = __shfl_xor_sync(~0u, give, st);
+                  if (up) pw[c][e] = got;
+                  else pw[c + st][e] = got;
+                }
               }
-              *reinterpret_cast<uint4*>(stage + lane * C::STAGE + (u ^ (lane & (CH - 1))) * 16) =
-                  make_uint4(pw[0], pw[1], pw[2], pw[3]);
-            }
-            __syncwarp();
-            uint4 v[CH];
-#pragma unroll
-            for (int k = 0; k < CH; ++k) {
-              const int rr = k * (32 / CH) + lane / CH;
-              v[k] = *reinterpret_cast<const uint4*>(stage + rr * C::STAGE +
-                                                     ((lane % CH) ^ (rr & (CH - 1))) * 16);
             }
 #pragma unroll
-            for (int k = 0; k < CH; ++k)
-              if (to[k]) *reinterpret_cast<uint4*>(to[k] + d) = v[k];
-            __syncwarp();
+            for (int k = 0; k < 4; ++k)
+              if (to[k])
+                *reinterpret_cast<uint4*>(to[k] + d) =
+                    make_uint4(pw[k][0], pw[k][1], pw[k][2], pw[k][3]);
           }
         } else {
           float* part = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + pc.slot) * C::PARTIAL +
@@ -805,9 +794,6 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             }
           }
         }
-        fence_async_smem();
-        bar_sync<128>(4 + wg);
-        if (ok && (tid & 127) == 0) mbar_arrive(&empty[vslot]);
         const float2 nan = unpack2(add2(nan2[0], nan2[1]));
         const bool odd = row && mine > 0 && ok && !(nan.x + nan.y == 0.f);
         again |= odd;

@@ -247,16 +247,6 @@ __device__ __forceinline__ bool block_any(bool v) {
   return r != 0;
 }
 
-// barrier `id` of N threads, some of which only say that they have come
-template <int N>
-__device__ __forceinline__ void bar_sync(int id) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void bar_arrive(int id) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory");
-}
-
 template <int ID, int N>
 __device__ __forceinline__ void named_sync() {
   asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
