@@ -177,6 +177,15 @@ int* err_of(const OptTensor& err, int device) {
   return static_cast<int*>(flag_of(device).data_ptr());
 }
 
+// n elements of a one-dimensional tensor from `first` on, without the dispatcher's way around
+Tensor part_of(const Tensor& t, int64_t first, int64_t n) {
+  Tensor v = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(),
+                                                      t.dtype());
+  v.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  v.unsafeGetTensorImpl()->set_storage_offset(first);
+  return v;
+}
+
 std::vector<Tensor> build_slots(const Tensor& kv_lens, const Tensor& new_lens,
                                 const Tensor& block_table, const Tensor& free_pages,
                                 const Tensor& free_pos, int64_t page_size, int64_t num_tokens,
@@ -202,9 +211,11 @@ std::vector<Tensor> build_slots(const Tensor& kv_lens, const Tensor& new_lens,
   if (c10::cuda::current_device() != dev) guard.set_index(dev);
   at::AutoDispatchBelowAutograd below;
   // one allocation for the five results
-  const int64_t sizes[5] = {batch + 1, num_tokens, num_tokens, batch, 1};
-  Tensor buf = at::empty({2 * batch + 2 + 2 * num_tokens}, block_table.options());
-  std::vector<Tensor> out = at::split_with_sizes(buf, at::IntArrayRef(sizes, 5));
+  const Tensor buf = at::empty({2 * batch + 2 + 2 * num_tokens}, block_table.options());
+  std::vector<Tensor> out{part_of(buf, 0, batch + 1), part_of(buf, batch + 1, num_tokens),
+                          part_of(buf, batch + 1 + num_tokens, num_tokens),
+                          part_of(buf, batch + 1 + 2 * num_tokens, batch),
+                          part_of(buf, 2 * batch + 1 + 2 * num_tokens, 1)};
   int32_t* p = static_cast<int32_t*>(buf.data_ptr());
   check_status(g_lib.build_slots((int)batch, kv, nw, table,
                                  batch < 2 ? columns : block_table.stride(0), (int)columns, pages,

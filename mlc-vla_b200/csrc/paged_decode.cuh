@@ -21,7 +21,8 @@
 // 8 exponentials a thread, so one warpgroup hides behind the loads.
 //
 // Work split: the tiles of all (request, kv head) units are numbered in one row and every CTA takes
-// an equal, contiguous share, whatever the lengths are. A unit that lies in several CTAs leaves
+// an equal, contiguous share, whatever the lengths are; when that is only a few tiles, as many CTAs as
+// there are take pieces of whole units instead. A unit that lies in several CTAs leaves
 // partials (unnormalised sums, M, l) that a second kernel joins in the order of the CTAs, so results
 // do not depend on timing.
 //
@@ -108,6 +109,8 @@ __global__ void __launch_bounds__(32) paged_rows_kernel(DecodeArgs a) {
 
 constexpr int kDecTile = 128;          // keys per tile
 constexpr int kDecThreads = 192;
+constexpr int kWholeTiles = 4;         // pieces of up to so many tiles keep to one unit
+constexpr int kWholeTries = 2;         // lengths tried: the least that could do, and one more
 constexpr float kDecGrow = 4.f;        // M is raised when it would grow by more than 2^4
 
 template <int HD, int NH>
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
       p_full[2], pv_done[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ float s_red[2][4][NH], s_qa[NH], s_l[4][NH];
-  __shared__ int s_scan[kDecThreads / 32], s_begin, s_total, s_at[3];
+  __shared__ int s_scan[1 + kWholeTries][kDecThreads / 32], s_begin, s_total, s_whole, s_rem, s_at[3];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.heads / a.cache.kv_heads, chunks = (group + NH - 1) / NH;
   const int subs = a.cache.kv_heads * chunks;
@@ -245,40 +248,79 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
   {
     const int per = (a.batch + kDecThreads - 1) / kDecThreads;
     const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b)
-      mine += (int)(((int64_t)held_len(a, b, cta == 0) + kDecTile - 1) / kDecTile) * subs;
-    int inc = mine;
+    auto tiles_of = [&](int b, bool report) {
+      return (int)(((int64_t)held_len(a, b, report) + kDecTile - 1) / kDecTile);
+    };
+    int mine[1 + kWholeTries] = {};  // tiles; and CTAs of whole pieces of each length tried
+    for (int b = b0; b < b1; ++b) mine[0] += tiles_of(b, cta == 0) * subs;
+    // sums of the first n numbers over the threads before this one, and over all
+    int before[1 + kWholeTries], all[1 + kWholeTries];
+    auto scan = [&](int from, int to) {
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(~0u, inc, d);
-      if (lane >= d) inc += up;
-    }
-    if (lane == 31) s_scan[warp] = inc;
-    __syncthreads();
-    int before = inc - mine, total = 0;
+      for (int v = 0; v <= kWholeTries; ++v) {
+        if (v < from || v >= to) continue;
+        int inc = mine[v];
 #pragma unroll
-    for (int w = 0; w < kDecThreads / 32; ++w) {
-      if (w < warp) before += s_scan[w];
-      total += s_scan[w];
+        for (int d = 1; d < 32; d <<= 1) {
+          const int up = __shfl_up_sync(~0u, inc, d);
+          if (lane >= d) inc += up;
+        }
+        if (lane == 31) s_scan[v][warp] = inc;
+        before[v] = inc - mine[v];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v <= kWholeTries; ++v) {
+        if (v < from || v >= to) continue;
+        all[v] = 0;
+#pragma unroll
+        for (int w = 0; w < kDecThreads / 32; ++w) {
+          if (w < warp) before[v] += s_scan[v][w];
+          all[v] += s_scan[v][w];
+        }
+      }
+    };
+    scan(0, 1);
+    const int total = all[0], most = (total + ctas - 1) / ctas;
+    int whole = 0, x0 = Shares<int>(total, ctas).begin(cta, total), b_before = before[0], b_mine = mine[0];
+    if (most <= kWholeTiles) {
+      // Few tiles: pieces of `whole` tiles that never cross from one unit into another, if there
+      // are CTAs enough, as beginning and ending a unit costs more than a tile or two.
+      for (int b = b0; b < b1; ++b) {
+        const int nt = tiles_of(b, false);
+#pragma unroll
+        for (int v = 0; v < kWholeTries; ++v) mine[1 + v] += subs * ((nt + most + v - 1) / (most + v));
+      }
+      scan(1, 1 + kWholeTries);
+#pragma unroll
+      for (int v = kWholeTries - 1; v >= 0; --v)
+        if (all[1 + v] <= ctas) {
+          whole = most + v;
+          x0 = cta < all[1 + v] ? cta : -1;
+          b_before = before[1 + v];
+          b_mine = mine[1 + v];
+        }
     }
-    const int x0 = Shares<int>(total, ctas).begin(cta, total);
     if (tid == 0) {
       s_begin = x0;
       s_total = total;
+      s_whole = total > 0 ? whole : 0;
+      s_rem = 0;
     }
-    if (x0 >= before && x0 < before + mine) {
-      int x = x0 - before;
-      int b = b0;
-      for (;; ++b) {
-        const int nt = (int)(((int64_t)held_len(a, b, false) + kDecTile - 1) / kDecTile);
-        if (x < nt * subs) {
+    __syncthreads();
+    if (x0 >= b_before && x0 < b_before + b_mine) {
+      int x = x0 - b_before;
+      for (int b = b0;; ++b) {
+        const int nt = tiles_of(b, false), each = whole ? (nt + whole - 1) / whole : nt;
+        if (x < each * subs) {
           s_at[0] = b;
-          s_at[1] = x / nt;
-          s_at[2] = x % nt;
+          s_at[1] = x / each;
+          s_at[2] = x % each * (whole ? whole : 1);
+          s_rem = whole ? min(whole, nt - s_at[2])
+                        : Shares<int>(total, ctas).begin(cta + 1, total) - x0;
           break;
         }
-        x -= nt * subs;
+        x -= each * subs;
       }
     }
     // requests without tokens: zeros
@@ -296,9 +338,9 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int total = s_total;
-  const Shares<int> shares(total, ctas);
-  DecWalk w{a, subs, s_at[0], s_at[1], s_at[2], shares.begin(cta + 1, total) - s_begin, 0, 0, 0};
+  const Shares<int> shares(s_total, ctas);
+  const int whole_tiles = s_whole;
+  DecWalk w{a, subs, s_at[0], s_at[1], s_at[2], s_rem, 0, 0, 0};
 
   if (warp == 0) {
     // ---- producer: one lane per box ----
@@ -691,7 +733,8 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
             part[NH * HD + NH + h] = l[h];
           }
         if (w.t0 == 0) {
-          meta = DecMeta{w.b, h0, nh, shares.owner(x + w.nt - 1) - cta + 1};
+          meta = DecMeta{w.b, h0, nh, whole_tiles ? (w.nt + whole_tiles - 1) / whole_tiles
+                                                  : shares.owner(x + w.nt - 1) - cta + 1};
         }
       }
       x += w.take;

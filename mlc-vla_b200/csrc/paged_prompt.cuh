@@ -223,6 +223,10 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
   const int group = a.heads / a.kv_heads, span = NQ * tok;
   const int ctas = gridDim.x, cta = blockIdx.x;
   pdl_trigger();  // every CTA of this grid is resident at once: the joining blocks may queue up
+  for (int b = tid; b < a.batch; b += C::THREADS) {  // read below, one after the other
+    pf_l1(a.cu_k + b);
+    if (a.prefix) pf_l1(a.prefix + b);
+  }
 
   if (tid == 0) {
     for (int i = 0; i < SLOTS; ++i) {
@@ -292,13 +296,13 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         if (s_tiles[mid] <= g0) lo = mid; else hi = mid;
       }
       t = g0 - s_tiles[lo];
-      for (b = lo * per; t >= (nt = tiles_of(b)); ++b) t -= nt;
+      for (b = lo * per; t >= (nt = tiles_of(b)) && b + 1 < a.batch; ++b) t -= nt;
       seq.load(a, b);
     }
     const int bg = b, tg = t;
     int64_t sum = 0;
     auto steps_of_next = [&]() {     // what tile (b, t) counts for, and on to the one behind it
-      while (t >= nt) {
+      while (t >= nt && b + 1 < a.batch) {
         t = 0;
         nt = tiles_of(++b);
         if (nt > 0) seq.load(a, b);
