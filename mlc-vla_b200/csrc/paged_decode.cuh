@@ -109,8 +109,8 @@ __global__ void __launch_bounds__(32) paged_rows_kernel(DecodeArgs a) {
 
 constexpr int kDecTile = 128;          // keys per tile
 constexpr int kDecThreads = 192;
-constexpr int kWholeTiles = 4;         // pieces of up to so many tiles keep to one unit
-constexpr int kWholeTries = 2;         // lengths tried: the least that could do, and one more
+constexpr int kWholeTiles = 8;         // pieces of up to so many tiles keep to one unit
+constexpr int kWholeTries = 4;         // lengths tried: the least that could do, and some more
 constexpr float kDecGrow = 4.f;        // M is raised when it would grow by more than 2^4
 
 template <int HD, int NH>
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
       scan(1, 1 + kWholeTries);
 #pragma unroll
       for (int v = kWholeTries - 1; v >= 0; --v)
-        if (all[1 + v] <= ctas) {
+        if (all[1 + v] <= ctas && v <= 1 + most / 2) {
           whole = most + v;
           x0 = cta < all[1 + v] ? cta : -1;
           b_before = before[1 + v];
