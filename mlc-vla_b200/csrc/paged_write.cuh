@@ -14,6 +14,7 @@
 #pragma once
 
 #include "paged_common.cuh"
+#include "paged_tc.cuh"
 
 namespace pi0 {
 namespace paged {
@@ -40,18 +41,14 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float((uint32_t)(max(x, -64) + 127) << 23);
 }
 
-// codes of eight values times `inv`; an infinity (only where `odd`) becomes NaN, as it has no code
-__device__ __forceinline__ uint2 to_e4m3x8(const float (&v)[8], float inv, bool odd) {
+// codes of eight values times `inv`
+__device__ __forceinline__ uint2 to_e4m3x8(const float (&v)[8], float inv) {
+  const uint64_t inv2 = pack2(inv, inv);
   __align__(8) uint16_t o[4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    float x = v[2 * u] * inv, y = v[2 * u + 1] * inv;
-    if (odd) {
-      if (isinf(x)) x = NAN;
-      if (isinf(y)) y = NAN;
-    }
-    o[u] = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-  }
+  for (int u = 0; u < 4; ++u)
+    o[u] = __nv_cvt_float2_to_fp8x2(unpack2(mul2(pack2(v[2 * u], v[2 * u + 1]), inv2)),
+                                    __NV_SATFINITE, __NV_E4M3);
   return *reinterpret_cast<uint2*>(o);
 }
 
@@ -62,21 +59,29 @@ __device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
   for (int i = 0; i < 8; ++i) x[i] = Tr<T>::f(e[i]);
 }
 
-// Magnitudes of 16-bit floats order like their bits below the sign, so the largest of a vector is an
-// integer maximum of pairs; from the type's infinity up they are no numbers.
+// Largest magnitudes of two 16-bit floats at a time; a NaN stays. Without a sign they order like their
+// bits, so lanes compare them as whole numbers: from the type's infinity up they are no numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (Tr<T>::kBf16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
 __device__ __forceinline__ uint32_t max_bits(uint32_t m, uint4 v) {
-  m = __vmaxu2(m, v.x & 0x7fff7fffu);
-  m = __vmaxu2(m, v.y & 0x7fff7fffu);
-  m = __vmaxu2(m, v.z & 0x7fff7fffu);
-  return __vmaxu2(m, v.w & 0x7fff7fffu);
+  const uint32_t a = max2<T>(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu);
+  const uint32_t b = max2<T>(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu);
+  return max2<T>(m, max2<T>(a, b));
 }
 // the same, of the numbers only
+template <typename T>
 __device__ __forceinline__ uint32_t max_bits_finite(uint32_t m, uint4 v, uint32_t inf) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
-    m = __vmaxu2(m, (lo < inf ? lo : 0u) | (hi < inf ? hi << 16 : 0u));
+    m = max2<T>(m, (lo < inf ? lo : 0u) | (hi < inf ? hi << 16 : 0u));
   }
   return m;
 }
@@ -126,16 +131,17 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
     auto at = [&](int v) { return src + (v / vec) * tok_stride + (v % vec) * 8; };
     uint4 held[VECS];
     {
-      int t = g / vec, d = g % vec;
+      int d = g % vec;
+      const T* p = at(g);
+      const int64_t step = dt * tok_stride + dd * 8, wrap = tok_stride - vec * 8;
 #pragma unroll
       for (int i = 0; i < VECS; ++i) {
-        held[i] = g + i * lanes < nv ? *reinterpret_cast<const uint4*>(src + t * tok_stride + d * 8)
-                                     : make_uint4(0, 0, 0, 0);
-        t += dt;
+        held[i] = g + i * lanes < nv ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+        p += step;
         d += dd;
         if (d >= vec) {
           d -= vec;
-          ++t;
+          p += wrap;
         }
       }
     }
@@ -151,17 +157,17 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
     const float old = row > 0 ? *sp : 0.f;
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) m = max_bits(m, held[i]);
+    for (int i = 0; i < VECS; ++i) m = max_bits<T>(m, held[i]);
 #pragma unroll 1
     for (int v = g + VECS * lanes; v < nv; v += lanes)
-      m = max_bits(m, *reinterpret_cast<const uint4*>(at(v)));
+      m = max_bits<T>(m, *reinterpret_cast<const uint4*>(at(v)));
     m = reduce(m, 0);
     const bool odd = m >= kInf;
     if (odd) {
       m = 0;
 #pragma unroll 1
       for (int v = g; v < nv; v += lanes)
-        m = max_bits_finite(m, *reinterpret_cast<const uint4*>(at(v)), kInf);
+        m = max_bits_finite<T>(m, *reinterpret_cast<const uint4*>(at(v)), kInf);
       m = reduce(m, 1);
     }
     const uint16_t bits = (uint16_t)m;
@@ -174,26 +180,32 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
         for (int i = g; i < row * vec; i += lanes) {
           float v[8];
           load8(codes + (int64_t)i * 8, 1.f, v);
-          *reinterpret_cast<uint2*>(codes + (int64_t)i * 8) = to_e4m3x8(v, ratio, false);
+          *reinterpret_cast<uint2*>(codes + (int64_t)i * 8) = to_e4m3x8(v, ratio);
         }
       }
     }
     const float inv = 1.f / s;
     uint8_t* dst = codes + (int64_t)row * hd;
+    const int rest = odd ? 0 : VECS;  // first vector of a lane that is read (again)
+    if (!odd) {
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int v = g + i * lanes;
-      if (v < nv) {
-        float f[8];
-        unpack8<T>(held[i], f);
-        *reinterpret_cast<uint2*>(dst + (int64_t)v * 8) = to_e4m3x8(f, inv, odd);
+      for (int i = 0; i < VECS; ++i) {
+        const int v = g + i * lanes;
+        if (v < nv) {
+          float f[8];
+          unpack8<T>(held[i], f);
+          *reinterpret_cast<uint2*>(dst + v * 8) = to_e4m3x8(f, inv);
+        }
       }
     }
 #pragma unroll 1
-    for (int v = g + VECS * lanes; v < nv; v += lanes) {
+    for (int v = g + rest * lanes; v < nv; v += lanes) {
       float f[8];
       load8(at(v), f);
-      *reinterpret_cast<uint2*>(dst + (int64_t)v * 8) = to_e4m3x8(f, inv, odd);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (isinf(f[u])) f[u] = NAN;  // it has no code
+      *reinterpret_cast<uint2*>(dst + v * 8) = to_e4m3x8(f, inv);
     }
     meet();  // every lane has read the old scale, and s_max
     if (g == 0) *sp = s;
