@@ -18,7 +18,11 @@
 //
 // Bound by HBM: 2 bytes per key, kv head and dimension. Per tile of 128 keys and 256 dimensions
 // (64 KB, 1.5 µs of one SM's share of HBM) the MMAs are 16 instructions of N = 32 and the softmax
-// 8 exponentials a thread, so one warpgroup hides behind the loads.
+// 8 exponentials a thread, so one warpgroup hides behind the loads; narrower heads load faster and
+// get two or three CTAs per SM. Measured: 64 requests of 8192 tokens, 32 heads on 8 of 128, 171 us in
+// pages of 128 (6260 GB/s, 96 % of the measured copy rate) and 180 us in pages of 16; of lengths 1 to
+// 16384, 182 us (5970 GB/s). Short requests are bound by latency: one of 1005 tokens takes 10 us,
+// 32 of 700 to 1100 14 us.
 //
 // Work split: the tiles of all (request, kv head) units are numbered in one row and every CTA takes
 // an equal, contiguous share, whatever the lengths are; when that is only a few tiles, as many CTAs as
