@@ -548,6 +548,37 @@ def test_paged_in_a_graph_follows_its_inputs():
     paged.check()
 
 
+def test_paged_on_two_streams_at_once():
+    """Calls on different streams overlap: each has a workspace of its own, also beside prompts."""
+    from mlc_vla import paged
+
+    rng = np.random.default_rng(1)
+    work = []
+    for lens, page in (([1900, 10, 900, 77], 64), ([1000, 1200, 2000], 16)):
+        c, table, _ = filled(rng, lens, page, 1, 128)
+        q = rows(rng, len(lens), 8, 128, dtype="float16")
+        k = rows(rng, 2000, 1, 128, dtype="float16")
+        work.append((q, c, dev(table), dev(lens), rows(rng, 500, 8, 128, dtype="float16"), k,
+                     dev([0, 500]), dev([0, 2000])))
+
+    def calls(w):
+        return (paged.attention_paged(*w[:4]), paged.attention_prompt(w[4], w[5], w[5], *w[6:]),
+                paged.attention_paged(*w[:4]))
+
+    want = [calls(w) for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(30):
+        for s, w in zip(streams, work):
+            with torch.cuda.stream(s):
+                got.append(calls(w))
+    torch.cuda.synchronize()
+    paged.check()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
 def test_paged_nan_tokens_stay_with_their_request():
     from mlc_vla import paged
 
