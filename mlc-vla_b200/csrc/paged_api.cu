@@ -334,7 +334,9 @@ int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64
                cu_seqlens_k, prefix_lens, err, static_cast<float*>(workspace),
                scale * 1.4426950408889634f, batch, total_q, total_k,
                heads, kv_heads, head_dim};
-  if (prompt_tc(heads, kv_heads, head_dim) && total_k > 0) {
+  // The tensor-core form takes the largest product for the largest logit; a scale that turns the order
+  // round, or levels it, is not worth a step's time (3 % when the sign was looked at there).
+  if (prompt_tc(heads, kv_heads, head_dim) && total_k > 0 && a.c > 0.f) {
     int device;
     const int sms = sm_count(&device);
     if (!sms) return PI0_ERR_CUDA;

@@ -29,6 +29,8 @@
 // earlier keys take 58 us instead of 85 with a CTA per tile.
 #pragma once
 
+#include <type_traits>
+
 #include "paged_common.cuh"
 #include "paged_tc.cuh"
 
@@ -76,7 +78,8 @@ struct PromptKV {
 
 constexpr int kRowWarps = 4;
 
-// One warp per (token, head), for the head sizes without a tensor-core form.
+// One warp per (token, head), for the head sizes without a tensor-core form and scales that are not
+// positive.
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) prompt_rows_kernel(PromptArgs a) {
   const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           const int buf = job_of(j) & 1, load = (2 * done + k_unit(j)) * SPT;
 #pragma unroll
           for (int h = 0; h < SPT; ++h) {
-            if (!ok || !(ok = full_of(load + h))) return;
+            if (!ok || ((NQ == 1 || j == 0) && !(ok = full_of(load + h)))) return;
             tc_fence_after();
             const int slot = (load + h) % SLOTS;
             const uint64_t da = tc::desc_sw128(qs + h * (HD / 64 / SPT) * 16384);
@@ -534,7 +537,10 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         };
         auto pv = [&](int j) {
           const int job = job_of(j), buf = job & 1, load = (2 * done + v_unit(j, take)) * SPT;
-          // V is there before the weights are; these come in two halves of the keys
+          // The keys of the logits behind this product, and V, are there before the weights are, which
+          // come in two halves of the keys. Waiting for them here takes nothing from between the
+          // products.
+          if (NQ == 2 && j + 1 < take && !(ok = full_of(2 * done + k_unit(j + 1)))) return;
 #pragma unroll
           for (int h = 0; h < SPT; ++h)
             if (!ok || !(ok = full_of(load + h))) return;
@@ -612,23 +618,21 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         // keys below these need no mask in this warpgroup's rows
         const int clear = tq < pc.lq ? visible(tq, pc.lq, pc.lk, pc.prefix) : 0;
         float m = -INFINITY, l = 0.f;
-        for (int t = 0; t < take; ++t) {
+        // one step; the second pass has a copy of its own, to keep the first's code short
+        auto step = [&](int t, auto second) {
+          constexpr bool careful = decltype(second)::value;
           const int job = NQ == 2 ? 2 * (done + t) + wg : done + t, buf = job & 1;
           const int key0 = pc.key0 + t * kKeys;
           if (ok) ok = bar_wait(&s_full[buf], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
           ok = __all_sync(~0u, ok);
           if (ok) {
             tc_fence_after();
-            float s[128], c = a.c;
+            float s[128];
+            const float c = a.c;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
               tmem_ld32_async(tl + buf * kKeys + 32 * q, reinterpret_cast<uint32_t*>(s) + 32 * q);
             tmem_wait_ld();
-            if (c <= 0.f) {  // the largest logit is not the largest product: scale first
-#pragma unroll
-              for (int u = 0; u < 128; ++u) s[u] *= c;
-              c = 1.f;
-            }
             if (key0 + kKeys > clear) {
               const int lim = mine - key0;
 #pragma unroll
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (pass == 0 && lane == 0) mbar_arrive(&p_full[buf][0]);
+                if (!careful && lane == 0) mbar_arrive(&p_full[buf][0]);
               }
             }
             const float2 sums = unpack2(add2(sum0, sum1));
@@ -693,9 +697,10 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
+            if (!careful && lane == 0) mbar_arrive(&p_full[buf][1]);  // the other tile can wait, P·V not
             if (NQ == 2 && lane == 0) mbar_arrive(&turn[wg ^ 1]);
           }
-          if (pass == 1 && key0 + kKeys > pc.fewest) {
+          if (careful && key0 + kKeys > pc.fewest) {
             // V rows of this tile, by all softmax warps: values that are no numbers become zero;
             // s_bad keeps the first key of the request that lost one
             const int load = (2 * done + v_unit(t, take)) * SPT;
@@ -728,10 +733,15 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             named_sync<1, NQ * 128>();
           }
           __syncwarp();
-          if (ok && lane == 0) {
-            if (pass == 1) mbar_arrive(&p_full[buf][0]);  // only now is V what it should be
+          if (careful && ok && lane == 0) {  // only now is V what it should be
+            mbar_arrive(&p_full[buf][0]);
             mbar_arrive(&p_full[buf][1]);
           }
+        };
+        if (pass == 0) {
+          for (int t = 0; t < take; ++t) step(t, std::false_type{});
+        } else {
+          for (int t = 0; t < take; ++t) step(t, std::true_type{});
         }
         const int last = NQ == 2 ? 2 * (done + take - 1) + wg : done + take - 1;
         done += take;
