@@ -13,15 +13,16 @@
 // on two. Per step, 128 queries × 128 keys:
 //   * S = Q·Kᵀ, tcgen05 kind::f16, from shared memory into tensor memory;
 //   * a thread per row takes its 128 logits into registers, masks, exponentiates, and writes the
-//     weights back over the logits in the type of V; P·V may start on the first 64 of them;
+//     weights back over the logits in the type of V; P·V starts before the last of them;
 //   * O += P·V with P from tensor memory.
 // The products of a step take 512, 1024 and 2048 clocks with 64, 128 and 256 dimensions, the
 // exponentials 1024 (16 a clock), and each waits for the other: two tiles per CTA work in turns, one in
-// its exponentials while the other is in its products. What a step takes with 128 dimensions is 3500 to
-// 3900 clocks for two tiles (2048 of products): shared-memory reads of the operands compete with the
-// loads of K and V, and power lowers the clock. Measured: 8192 tokens, 32 heads on 8 of 128, all keys
-// 900 us (1220 TFLOP/s, 73 % of the measured 1661), causal 520 us (1055); 8 heads on 1 of 256, all
-// keys 401 us (1370).
+// its exponentials while the other is in its products. What a step takes with 128 dimensions is 3300 to
+// 3600 clocks for two tiles (2048 of products): from logits to logits a tile spends 600 on loading them
+// and their maximum, 1450 in its exponentials, 1100 in P·V and the next logits, whose reads of shared
+// memory compete with the loads of K and V, and the rest on handing over; power lowers the clock.
+// Measured: 8192 tokens, 32 heads on 8 of 128, all keys 828 us (1327 TFLOP/s, 80 % of the measured
+// 1661), causal 475 us (1156); 8 heads on 1 of 256, all keys 401 us (1370).
 //
 // Work split: the steps of all (tile, kv head) are numbered in one row, and every CTA takes an equal,
 // contiguous share, whatever the lengths are. What lies in several CTAs leaves partial sums that a
@@ -121,6 +122,9 @@ struct PromptCfg {
   static constexpr int SMEM = NQ * Q_TILE + SLOTS * SLOT + 1024;
   static constexpr int THREADS = 128 + NQ * 128;   // producer, MMA issuers (and an idle warp); softmax
   static constexpr int VKEYS = kKeys / SPT;         // keys of a V slot
+  // P·V starts on the first weights while the last are worked on: what is left then holds up the
+  // next logits. A half is the most where V comes in halves (96 against 64 of 128: 1 %).
+  static constexpr int FIRST = SPT == 1 ? 96 : 64;
   // tensor memory: two tiles of logits, each overlaid by its weights, then the sums
   static constexpr int O_COL = 256;
   // a partial: for each tile of rows the sums as [HD / 4][128 rows][4], then M and l of the rows
@@ -538,8 +542,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         auto pv = [&](int j) {
           const int job = job_of(j), buf = job & 1, load = (2 * done + v_unit(j, take)) * SPT;
           // The keys of the logits behind this product, and V, are there before the weights are, which
-          // come in two halves of the keys. Waiting for them here takes nothing from between the
-          // products.
+          // come in two parts: waiting for them here takes nothing from between the products.
           if (NQ == 2 && j + 1 < take && !(ok = full_of(2 * done + k_unit(j + 1)))) return;
 #pragma unroll
           for (int h = 0; h < SPT; ++h)
@@ -551,12 +554,13 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             tc_fence_after();
             const int slot = (load + h * (SPT - 1)) % SLOTS;
             const uint64_t dv = sdesc<128>(ring + slot * C::SLOT, 1024, C::VKEYS * 128) +
-                                (SPT == 1 ? 512 * h : 0);
-            const uint32_t tp = tm + buf * kKeys + 32 * h;
+                                (SPT == 1 ? C::FIRST * 8 * h : 0);
+            const uint32_t tp = tm + buf * kKeys + C::FIRST / 2 * h;
             const uint32_t more = (j | h) != 0;
             if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)  // 16 keys (2048 bytes of V rows) a step
+              for (int k = 0; k < (h == 0 ? C::FIRST : kKeys - C::FIRST) / 16; ++k)
+                // 16 keys, 2048 bytes of V rows, each
                 umma_f16_ta(to, tp + 8 * k, dv + 128 * k, id_o, k == 0 ? more : 1u);
               if (h == 1) umma_commit(&pv_done[buf]);
               if (h >= 2 - SPT) umma_commit(&empty[slot]);
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                 pw[u] = Tr<T>::pack(e0, e1);
               }
               tmem_st16(tl + buf * kKeys + 16 * q, pw);
-              if (q == 1) {  // the first 64 weights may go
+              if (q == C::FIRST / 32 - 1) {  // the first weights may go
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
