@@ -222,9 +222,9 @@ typedef struct pi0_kv8 {
  * [batch, max_pages] (row stride table_stride) behind the pages that a request holds already.
  * Writes cu_seqlens [batch + 1] (sums of new_lens), positions and slot_mapping [num_tokens] of the
  * packed new tokens (-1 slots for tokens behind the last request's), kv_lens_out [batch] and
- * free_pos_out [1], which may alias their inputs only if no other call reads these. A request that
- * its table row or the pool cannot hold is not admitted: its slots are -1, its length stays.
- * batch ≤ 16384. */
+ * free_pos_out [1]. These five may overlap neither one another nor the inputs, which are read while
+ * they are written (PI0_ERR_INVALID). A request that its table row or the pool cannot hold is not
+ * admitted: its slots are -1, its length stays. batch ≤ 16384. */
 int pi0_build_slots(int batch, const int32_t* kv_lens, const int32_t* new_lens,
                     int32_t* block_table, int64_t table_stride, int max_pages,
                     const int32_t* free_pages, int n_free, const int32_t* free_pos, int num_pages,

@@ -23,6 +23,13 @@ bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 bool dtype_ok(int dtype) { return dtype == PI0_F16 || dtype == PI0_BF16; }
 int launched() { return cudaGetLastError() == cudaSuccess ? PI0_OK : PI0_ERR_CUDA; }
 
+// n int32 numbers from p on
+struct Ints {
+  const int32_t* p;
+  int64_t n;
+  bool meets(const Ints& o) const { return n > 0 && o.n > 0 && p < o.p + o.n && o.p < p + n; }
+};
+
 // one 16-bit operand [tokens, heads, head_dim]: 16-byte vectors along the last dimension
 bool rows_ok(const void* p, int64_t tok, int64_t head) {
   return p && !off16(p) && tok > 0 && head > 0 && tok % 8 == 0 && head % 8 == 0;
@@ -251,6 +258,16 @@ int pi0_build_slots(int batch, const int32_t* kv_lens, const int32_t* new_lens,
       (num_tokens && (!positions || !slot_mapping)))
     return PI0_ERR_INVALID;
   if (batch > kSlotMaxBatch) return PI0_ERR_UNSUPPORTED;
+  // Blocks read the inputs at any time while others write the outputs.
+  const Ints in[] = {{kv_lens, batch}, {new_lens, batch}, {free_pages, n_free}, {free_pos, 1}};
+  const Ints out[] = {{cu_seqlens, (int64_t)batch + 1}, {positions, num_tokens},
+                      {slot_mapping, num_tokens}, {kv_lens_out, batch}, {free_pos_out, 1}};
+  for (const Ints& o : out) {
+    for (const Ints& i : in)
+      if (o.meets(i)) return PI0_ERR_INVALID;
+    for (const Ints& x : out)
+      if (&x != &o && o.meets(x)) return PI0_ERR_INVALID;
+  }
   const size_t smem = 2 * sizeof(int) * ((size_t)batch + 1);
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(build_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
