@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
     s_cu[0] = s_off[0] = 0;
     s_used = 0;
   }
+  __syncthreads();  // an empty batch meets no other barrier before these are read
 
   // a request's own numbers; a length below zero counts as zero, and one that its table row cannot
   // hold asks for no page
