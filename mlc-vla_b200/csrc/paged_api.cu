@@ -268,17 +268,20 @@ int pi0_build_slots(int batch, const int32_t* kv_lens, const int32_t* new_lens,
     for (const Ints& x : out)
       if (&x != &o && o.meets(x)) return PI0_ERR_INVALID;
   }
-  const size_t smem = 2 * sizeof(int) * ((size_t)batch + 1);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(build_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)smem) != cudaSuccess)
-    return PI0_ERR_CUDA;
+  int device;
+  const int sms = sm_count(&device);
+  if (!sms) return PI0_ERR_CUDA;
+  const auto smem = [](int n) { return (int)(2 * sizeof(int)) * (n + 1); };
+  // the limit of the largest batch, once: a limit per call could be lowered between another host
+  // thread's limit and launch
+  if (!allow_smem<build_slots_kernel>(device, smem(kSlotMaxBatch))) return PI0_ERR_CUDA;
   SlotArgs a{kv_lens, new_lens, block_table, table_stride, free_pages, free_pos, cu_seqlens,
              positions, slot_mapping, kv_lens_out, free_pos_out, err, batch, max_pages, n_free,
              num_pages, page_size, num_tokens};
   // two tokens a thread until one block per SM is reached
-  const int grid = std::max(1, std::min(148, (num_tokens + 2 * kSlotThreads - 1) / (2 * kSlotThreads)));
-  build_slots_kernel<<<grid, kSlotThreads, smem, stream>>>(a);
+  const int grid = std::max(1, std::min(sms, (int)((num_tokens + 2 * kSlotThreads - INT64_C(1)) /
+                                                   (2 * kSlotThreads))));
+  build_slots_kernel<<<grid, kSlotThreads, smem(batch), stream>>>(a);
   return launched();
 }
 

@@ -29,3 +29,43 @@ def test_slots_of_an_empty_batch(tokens):
     assert s.cu_seqlens.tolist() == [0] and s.kv_lens.numel() == 0 and s.free_pos.tolist() == [1]
     assert (s.slot_mapping == -1).all() and (s.positions == 0).all()
     assert len(s.slot_mapping) == len(s.positions) == tokens
+
+
+@pytest.mark.parametrize("batch", [6127, 6128, 6136, 6143, 6144, 7000, 16384])
+def test_slots_of_large_batches(batch):
+    """The sums of up to 16384 requests lie in shared memory, beyond its default limit from 6128 on."""
+    from mlc_vla import paged
+
+    rng = np.random.default_rng(batch)
+    page, columns = 4, 3
+    kv, new = rng.integers(0, 6, batch), rng.integers(0, 4, batch)
+    table = np.full((batch, columns), -1)
+    have, need = -(-kv // page), -(-(kv + new) // page) - -(-kv // page)
+    order = rng.permutation(int(have.sum() + need.sum()))
+    at = 0
+    for r in range(batch):
+        table[r, :have[r]] = order[at:at + have[r]]
+        at += have[r]
+    free, want = order[at:], table.copy()
+    cu = np.concatenate([[0], np.cumsum(new)])
+    first = np.cumsum(need) - need
+    positions, slots = [], []
+    for r in range(batch):
+        want[r, have[r]:have[r] + need[r]] = free[first[r]:first[r] + need[r]]
+        for p in range(kv[r], kv[r] + new[r]):
+            positions.append(p)
+            slots.append(want[r, p // page] * page + p % page)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = dev(table)
+    s = paged.build_slots(dev(kv), dev(new), got, dev(free), dev([0]), page, int(cu[-1]), err=err)
+    assert int(err.item()) == 0
+    for g, w in zip((got, *s), (want, cu, positions, slots, kv + new, [need.sum()])):
+        assert np.array_equal(g.cpu().numpy(), np.array(w))
+
+
+def test_slots_of_too_many_requests_are_refused():
+    from mlc_vla import paged
+
+    n = torch.zeros(16385, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        paged.build_slots(n, n, n[:, None].expand(16385, 1).contiguous(), n, n[:1], 8, 4)
