@@ -59,6 +59,8 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
   const int pos0 = max(0, *a.free_pos);
   const int avail = max(0, a.n_free - pos0);
   const int ps = a.page_size;
+  // tokens that a table row can hold and a length count
+  const int64_t room = min((int64_t)a.max_pages * ps, (int64_t)0x7fffffff);
   if (tid == 0) {
     s_cu[0] = s_off[0] = 0;
     s_used = 0;
@@ -77,7 +79,7 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
     const int64_t end = (int64_t)kv + nw;
     have = (int)(((int64_t)kv + ps - 1) / ps);
     need = 0;
-    if (end > (int64_t)a.max_pages * ps) code = PI0_PAGED_ERR_TABLE;
+    if (end > room) code = PI0_PAGED_ERR_TABLE;
     else need = (int)((end + ps - 1) / ps) - have;
     return code;
   };
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
   // admitted: the table row holds it and the pool has its pages. Offsets ascend, so of the
   // requests that need pages the admitted ones are the first ones.
   auto admitted = [&](int r, int kv, int nw) -> bool {
-    return (int64_t)kv + nw <= (int64_t)a.max_pages * ps &&
+    return (int64_t)kv + nw <= room &&
            (s_off[r + 1] == s_off[r] || s_off[r + 1] <= avail);
   };
   if (blockIdx.x == 0) {
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
       const int r = last_le(s_cu, a.batch, t);
       const int kv = max(a.kv_lens[r], 0), nw = max(a.new_lens[r], 0);
       const int have = (int)(((int64_t)kv + ps - 1) / ps);
-      pos = kv + (t - s_cu[r]);
+      pos = (int)((unsigned)kv + (unsigned)(t - s_cu[r]));  // wraps only where it is not admitted
       if (admitted(r, kv, nw)) {
         const int col = pos / ps;
         // a page that the request holds already stands in its table row; a new one is read from

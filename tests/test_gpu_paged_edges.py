@@ -69,3 +69,23 @@ def test_slots_of_too_many_requests_are_refused():
     n = torch.zeros(16385, dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError):
         paged.build_slots(n, n, n[:, None].expand(16385, 1).contiguous(), n, n[:1], 8, 4)
+
+
+def test_slots_of_lengths_beyond_31_bits():
+    """A table row may have room for more tokens than a length can count."""
+    from mlc_vla import paged
+
+    page, columns = 1 << 20, 2100
+    table = torch.zeros((2, columns), dtype=torch.int32, device="cuda")
+    kv = [(1 << 31) - 648, 3]
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    s = paged.build_slots(dev(kv), dev([1000, 2]), table, dev([5, 6, 7]), dev([0]), page, 1002, err=err)
+    assert int(err.item()) == 17
+    assert s.kv_lens.tolist() == [kv[0], 5] and s.free_pos.tolist() == [0]
+    assert (s.slot_mapping[:1000] == -1).all() and s.slot_mapping[1000:].tolist() == [3, 4]
+    assert not table.any()
+    # up to the last length that it can
+    err.zero_()
+    s = paged.build_slots(dev(kv), dev([647, 2]), table, dev([5, 6, 7]), dev([0]), page, 649, err=err)
+    assert int(err.item()) == 0 and s.kv_lens.tolist() == [(1 << 31) - 1, 5]
+    assert s.positions[:647].tolist() == list(range(kv[0], kv[0] + 647))
