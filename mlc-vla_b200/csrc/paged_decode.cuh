@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     scan(0, 1);
     const int total = all[0], most = (total + ctas - 1) / ctas;
     int whole = 0, x0 = Shares<int>(total, ctas).begin(cta, total), b_before = before[0], b_mine = mine[0];
-    if (most <= kWholeTiles) {
+    if (total > 0 && most <= kWholeTiles) {
       // Few tiles: pieces of `whole` tiles that never cross from one unit into another, if there
       // are CTAs enough, as beginning and ending a unit costs more than a tile or two.
       for (int b = b0; b < b1; ++b) {
@@ -308,13 +308,13 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     if (tid == 0) {
       s_begin = x0;
       s_total = total;
-      s_whole = total > 0 ? whole : 0;
+      s_whole = whole;
       s_rem = 0;
     }
     __syncthreads();
     if (x0 >= b_before && x0 < b_before + b_mine) {
       int x = x0 - b_before;
-      for (int b = b0;; ++b) {
+      for (int b = b0; b < b1; ++b) {
         const int nt = tiles_of(b, false), each = whole ? (nt + whole - 1) / whole : nt;
         if (x < each * subs) {
           s_at[0] = b;

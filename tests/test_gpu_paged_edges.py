@@ -89,3 +89,33 @@ def test_slots_of_lengths_beyond_31_bits():
     s = paged.build_slots(dev(kv), dev([647, 2]), table, dev([5, 6, 7]), dev([0]), page, 649, err=err)
     assert int(err.item()) == 0 and s.kv_lens.tolist() == [(1 << 31) - 1, 5]
     assert s.positions[:647].tolist() == list(range(kv[0], kv[0] + 647))
+
+
+# ---- attention over the cache ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("batch", [1, 3, 193, 1000])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 1, 256, 64), (4, 2, 128, 16), (40, 2, 64, 8),
+                                                     (3, 1, 72, 16)])
+def test_paged_batch_without_any_token(batch, heads, kv_heads, dim, page):
+    from mlc_vla import paged
+
+    c = paged.KVCache8.empty(2, page, kv_heads, dim)
+    for t in c:
+        t.view(torch.uint8).fill_(0x7F)
+    table = torch.full((batch, 3), -1, dtype=torch.int32, device="cuda")
+    q = torch.ones((batch, heads, dim), dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, 7.0)
+    paged.attention_paged(q, c, table, dev(np.zeros(batch, np.int32)), out=out)
+    paged.check()
+    assert not out.any()
+    # the same without a token but in the last request
+    lens = np.zeros(batch, np.int32)
+    lens[-1] = 1
+    c.k.view(torch.uint8).zero_()
+    c.v.view(torch.uint8).fill_(0x38)  # 1.0
+    c.k_scale.fill_(1.0)
+    c.v_scale.fill_(0.5)
+    table[-1] = 1
+    paged.attention_paged(q, c, table, dev(lens), out=out)
+    paged.check()
+    assert not out[:-1].any() and (out[-1] == 0.5).all()
