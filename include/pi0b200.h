@@ -237,8 +237,10 @@ int pi0_build_slots(int batch, const int32_t* kv_lens, const int32_t* new_lens,
  * scale of a page and head is the smallest power of two, not below 2^-64, with which the largest
  * magnitude of its tokens fits into ±448; tokens that join a page (kv_lens: tokens cached before)
  * keep or raise its scale, and codes already there are rounded to a raised one. Infinities and NaN
- * are stored as NaN and do not count for the scale. Tokens with slot -1 are left out. max_new: the
- * most new tokens of one request, which sizes the launch (a larger request is still written). */
+ * are stored as NaN and do not count for the scale. Tokens with slot -1 are left out: their rows keep
+ * their codes. So are, reported, those whose slot is not their row of the page that the request's
+ * first other token there names. max_new: the most new tokens of one request, which sizes the launch
+ * (a larger request is still written). */
 int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_head_stride,
                  const void* v, int64_t v_token_stride, int64_t v_head_stride, int num_tokens,
                  int batch, const int32_t* cu_seqlens, const int32_t* kv_lens,

@@ -5,7 +5,9 @@
 // exact, so the only rounding is e4m3's, to nearest even. Tokens that join a page which holds some
 // already keep or raise its scale; when it rises, the codes there are rounded once more, to the
 // new step (exact for every code that stays above e4m3's subnormals). An infinity or a NaN has no
-// finite code: it is stored as NaN and does not count for the scale.
+// finite code: it is stored as NaN and does not count for the scale. Neither does a token that is
+// left out: one without a slot, or whose slot is not its row of the page that the first token with
+// a slot of its own row names.
 //
 // Bound by HBM: 2 bytes read and 1 written per element, plus the scales. A (page, kv head) is held in
 // the registers of the few warps that take it, up to 16 vectors of 16 bytes a lane: one pass over the
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
   const int ps = c.page_size, hd = c.head_dim, vec = hd / 8, kinds = 2 * c.kv_heads;
   const int lanes = 32 * a.warps, units = kWriteWarps / a.warps;  // of a unit, of a block
   const int unit = threadIdx.x / lanes, g = threadIdx.x % lanes;
-  __shared__ uint32_t s_max[2][kWriteWarps];
+  __shared__ uint32_t s_max[3][kWriteWarps];
   const int r = blockIdx.z;
   const int start = max(a.kv_lens[r], 0);
   const int t0 = min(max(a.cu[r], 0), a.tokens), t1 = min(max(a.cu[r + 1], t0), a.tokens);
@@ -109,8 +111,8 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
     if (a.warps == 1) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + unit), "r"(lanes) : "memory");
   };
-  auto reduce = [&](uint32_t m, int slot) -> uint32_t {
-    m = __reduce_max_sync(~0u, max(m & 0xffffu, m >> 16));
+  auto most = [&](uint32_t m, int slot) -> uint32_t {
+    m = __reduce_max_sync(~0u, m);
     if (a.warps > 1) {
       if ((threadIdx.x & 31) == 0) s_max[slot][threadIdx.x >> 5] = m;
       meet();
@@ -148,31 +150,49 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
         }
       }
     }
-    const int slot = a.slots[tok];
-    const int page = slot / ps;
-    const bool none = slot < 0;  // not admitted to the pool
-    const bool bad = !none && (page >= c.num_pages || slot % ps != row);
-    if (bad && g == 0) set_err(a.err, PI0_PAGED_ERR_PAGE);
-    if (none || bad) continue;   // the same for all lanes of the unit
-    const int64_t ph = (int64_t)page * c.kv_heads + h;
-    float* sp = (kind ? c.vs : c.ks) + ph;
-    uint8_t* codes = (kind ? c.v : c.k) + ph * ps * hd;
-    const float old = row > 0 ? *sp : 0.f;
+    // Every token at its row of one page, which is the first's: looked at while the vectors are on
+    // their way. If not, the unit takes the path of infinities, which looks at each token.
+    const int* slots = a.slots + tok;
+    const int pool = c.num_pages * ps;
+    int slot0 = slots[0];  // of the run's first token
+    bool odd = (unsigned)slot0 >= (unsigned)pool || slot0 % ps != row;
+    float* scales = kind ? c.vs : c.ks;
+    auto scale_at = [&]() { return scales + (int64_t)(slot0 / ps) * c.kv_heads + h; };
+    float old = row > 0 && !odd ? *scale_at() : 0.f;
+    for (int i = g; i < n; i += lanes) odd |= slots[i] != slot0 + i;
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) m = max_bits<T>(m, held[i]);
 #pragma unroll 1
     for (int v = g + VECS * lanes; v < nv; v += lanes)
       m = max_bits<T>(m, *reinterpret_cast<const uint4*>(at(v)));
-    m = reduce(m, 0);
-    const bool odd = m >= kInf;
+    m = most(max(m & 0xffffu, m >> 16) | (odd ? 0x10000u : 0u), 0);
+    odd = m >= kInf;
     if (odd) {
+      uint32_t left = 0;  // n − i for the first token i whose slot is its row of a page
+#pragma unroll 1
+      for (int i = g; i < n; i += lanes)
+        if ((unsigned)slots[i] < (unsigned)pool && slots[i] % ps == row + i)
+          left = max(left, (uint32_t)(n - i));
+      left = most(left, 1);
+      slot0 = left ? slots[n - left] - (int)(n - left) : -1;
+#pragma unroll 1
+      for (int i = g; i < n; i += lanes)
+        if (slots[i] >= 0 && (!left || slots[i] != slot0 + i)) set_err(a.err, PI0_PAGED_ERR_PAGE);
       m = 0;
 #pragma unroll 1
       for (int v = g; v < nv; v += lanes)
-        m = max_bits_finite<T>(m, *reinterpret_cast<const uint4*>(at(v)), kInf);
-      m = reduce(m, 1);
+        if (left && slots[v / vec] == slot0 + v / vec)
+          m = max_bits_finite<T>(m, *reinterpret_cast<const uint4*>(at(v)), kInf);
+      m = most(max(m & 0xffffu, m >> 16), 2);
+      if (!left) {  // the same for all lanes of the unit
+        meet();     // they have read s_max
+        continue;
+      }
+      if (row > 0) old = *scale_at();
     }
+    float* sp = scale_at();
+    uint8_t* codes = (kind ? c.v : c.k) + (sp - scales) * ps * hd;
     const uint16_t bits = (uint16_t)m;
     float s = pow2_scale(Tr<T>::f(*reinterpret_cast<const T*>(&bits)));
     if (row > 0) {
@@ -203,6 +223,7 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
     }
 #pragma unroll 1
     for (int v = g + rest * lanes; v < nv; v += lanes) {
+      if (odd && slots[v / vec] != slot0 + v / vec) continue;
       float f[8];
       load8(at(v), f);
 #pragma unroll

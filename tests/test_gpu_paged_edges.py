@@ -91,6 +91,98 @@ def test_slots_of_lengths_beyond_31_bits():
     assert s.positions[:647].tolist() == list(range(kv[0], kv[0] + 647))
 
 
+# ---- the cache ------------------------------------------------------------------------------------
+
+def e4m3_of(x):
+    return torch.as_tensor(x, dtype=torch.float32).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+
+
+def joined(codes, scales, x, cu, lens, slots, page):
+    """Codes (bytes) [pages, heads, page, dim] and scales after the tokens joined, token by token: a
+    token is written if its slot is its row of a page of the pool, and of the page that the first
+    such token of its run names. The scale is that of the written tokens and of the rows held before."""
+    codes, scales, reported = codes.copy(), scales.copy(), False
+    number = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    for r, start in enumerate(lens):
+        t = cu[r]
+        while t < cu[r + 1]:
+            row = (start + t - cu[r]) % page
+            n = min(page - row, cu[r + 1] - t)
+            own = [i for i in range(n) if 0 <= slots[t + i] < len(codes) * page
+                   and slots[t + i] % page == row + i]
+            p = slots[t + own[0]] // page if own else -1
+            put = [i for i in own if slots[t + i] // page == p]
+            reported |= any(slots[t + i] >= 0 and i not in put for i in range(n))
+            for h in range(codes.shape[1] if put else 0):
+                part = x[[t + i for i in put], h]
+                top = np.abs(part[np.isfinite(part)]).max(initial=0.0)
+                s = 2.0 ** -64
+                while top > 448.0 * s:
+                    s *= 2.0
+                if row:
+                    s = max(s, scales[p, h])
+                    if s > scales[p, h]:
+                        codes[p, h, :row] = e4m3_of(number[codes[p, h, :row]] * (scales[p, h] / s))
+                scales[p, h] = s
+                for i, values in zip(put, part):
+                    codes[p, h, row + i] = e4m3_of(np.where(np.isfinite(values), values, np.nan) / s)
+            t += n
+    return codes, scales, reported
+
+
+@pytest.mark.parametrize("page,heads,dim,dtype", [
+    (16, 2, 64, "float16"), (64, 1, 256, "bfloat16"), (128, 2, 256, "float16"), (24, 1, 72, "bfloat16"),
+    (256, 1, 128, "float16"), (8, 3, 128, "bfloat16")])
+@pytest.mark.parametrize("held", [0, 5])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_cache_takes_each_token_by_its_own_slot(page, heads, dim, dtype, held, infinite):
+    from mlc_vla import paged
+
+    rng = np.random.default_rng(page + dim + held)
+    new, pages = [page + 3, 2 * page, 4, 3, 1], 12
+    lens = [held, held, 0, held, page - 1]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    slots, at = [], 0
+    for r, n in enumerate(new):
+        first = lens[r]
+        for p in range(first, first + n):
+            slots.append((at + p // page) * page + p % page)
+        at += -(-(first + n) // page)
+    assert at <= pages
+    right, slots = list(slots), np.array(slots)
+    slots[2] = -1                       # within a page
+    slots[cu[1]] = -1                   # the first token of a page's run
+    slots[cu[1] + 2] = slots[cu[1] + 3]   # another's row
+    slots[cu[2] - 1] = -1               # the last token of a page's run
+    slots[cu[2] + 1] += page            # its row of another page
+    slots[cu[3]:cu[4]] = -1             # a request that was not admitted
+    x = [rng.standard_normal((cu[-1], heads, dim)) * np.exp(rng.standard_normal((cu[-1], heads, 1)))
+         for _ in range(2)]
+    for y in x:
+        y[[2, cu[1], cu[2] - 1]] *= 1000.0  # what is left out must not count for the scale
+        if infinite:
+            y[1, 0, 3], y[cu[1] + 1, 0, 0], y[cu[1], 0, 0] = np.inf, np.nan, -np.inf
+    x = [torch.as_tensor(y).to(getattr(torch, dtype)).cuda() for y in x]
+    codes = rng.integers(0, 0x7E, (2, pages, heads, page, dim)).astype(np.uint8)
+    scales = 2.0 ** rng.integers(-12, -6, (2, pages, heads))
+    c = paged.KVCache8(*(torch.as_tensor(a).cuda().view(torch.float8_e4m3fn) for a in codes),
+                       *(torch.as_tensor(a).float().cuda() for a in scales))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    paged.write_kv(c, *x, dev(cu), dev(lens), dev(slots), max_new=max(new), err=err)
+    for y, got, got_scale, a, b in zip(x, (c.k, c.v), (c.k_scale, c.v_scale), codes, scales):
+        want, want_scale, reported = joined(a, b, y.double().cpu().numpy(), cu, lens, slots, page)
+        assert reported and int(err.item()) == 19
+        assert np.array_equal(got_scale.cpu().double().numpy(), want_scale)
+        got = got.view(torch.uint8).cpu().numpy()
+        nan = (got & 0x7F) == 0x7F
+        assert np.array_equal(nan, (want & 0x7F) == 0x7F)
+        assert np.array_equal(got[~nan], want[~nan])
+    # all in their places: nothing is reported
+    err.zero_()
+    paged.write_kv(c, *x, dev(cu), dev(lens), dev(right), max_new=max(new), err=err)
+    assert int(err.item()) == 0
+
+
 # ---- attention over the cache ---------------------------------------------------------------------
 
 @pytest.mark.parametrize("batch", [1, 3, 193, 1000])
