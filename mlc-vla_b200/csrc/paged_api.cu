@@ -292,13 +292,14 @@ int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_hea
                  pi0_stream_t stream) {
   if (!dtype_ok(dtype) || num_tokens < 0 || batch < 0 || max_new < 0 || !cache_ok(cache))
     return PI0_ERR_INVALID;
-  if (num_tokens == 0 || batch == 0 || max_new == 0) return PI0_OK;
+  if (num_tokens == 0 || batch == 0) return PI0_OK;
+  max_new = std::max(1, std::min(max_new, num_tokens));  // a size of the launch, whatever it says
   if (!rows_ok(k, k_token_stride, k_head_stride) || !rows_ok(v, v_token_stride, v_head_stride) ||
       !cu_seqlens || !kv_lens || !slot_mapping)
     return PI0_ERR_INVALID;
   if (batch > 65535 || cache->kv_heads > 32767) return PI0_ERR_UNSUPPORTED;
   // as many vectors a lane, then as many warps, as hold a (page, kv head) in registers
-  const int64_t vecs = (int64_t)std::min(cache->page_size, std::min(max_new, num_tokens)) *
+  const int64_t vecs = (int64_t)std::min(cache->page_size, max_new) *
                        (cache->head_dim / 8);
   const int held = vecs <= 32 ? 1 : vecs <= 128 ? 4 : 16;
   int warps = 1;
@@ -306,8 +307,7 @@ int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_hea
   WriteArgs a{{k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride},
               cu_seqlens, kv_lens, slot_mapping, err, cache_of(cache), num_tokens, warps};
   // n tokens touch at most ⌈(n − 1)/page⌉ + 1 pages; a request with more than max_new loops
-  const int64_t pages = (std::min(max_new, num_tokens) + (int64_t)cache->page_size - 2) /
-                            cache->page_size + 1;
+  const int64_t pages = (max_new + (int64_t)cache->page_size - 2) / cache->page_size + 1;
   const int units = kWriteWarps / warps;
   const int64_t blocks = (pages * 2 * cache->kv_heads + units - 1) / units;
   const dim3 grid((unsigned)std::min<int64_t>(blocks, INT_MAX), 1, batch);

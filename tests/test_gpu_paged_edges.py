@@ -183,6 +183,22 @@ def test_cache_takes_each_token_by_its_own_slot(page, heads, dim, dtype, held, i
     assert int(err.item()) == 0
 
 
+@pytest.mark.parametrize("most", [0, 1, 1000])
+def test_cache_writes_whatever_the_launch_was_sized_for(most):
+    from mlc_vla import paged
+
+    rng = np.random.default_rng(0)
+    k, v = (torch.as_tensor(rng.standard_normal((37, 2, 64))).half().cuda() for _ in range(2))
+    cu, lens, slots = dev([0, 20, 37]), dev([0, 0]), dev(np.r_[16:36, 48:65])
+    got, want = ([t.zero_() for t in paged.KVCache8.empty(6, 16, 2, 64)] for _ in range(2))
+    paged.write_kv(paged.KVCache8(*got), k, v, cu, lens, slots, max_new=most)
+    paged.write_kv(paged.KVCache8(*want), k, v, cu, lens, slots)
+    paged.check()
+    for g, w in zip(got, want):
+        assert w.view(torch.uint8).any()
+        assert torch.equal(g.view(torch.uint8), w.view(torch.uint8))
+
+
 # ---- attention over the cache ---------------------------------------------------------------------
 
 @pytest.mark.parametrize("batch", [1, 3, 193, 1000])
