@@ -217,8 +217,9 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
       p_full[2], pv_done[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ float s_red[2][4][NH], s_qa[NH], s_l[4][NH];
-  __shared__ int s_scan[1 + kWholeTries][kDecThreads / 32], s_begin, s_total, s_whole, s_rem, s_at[3];
+  __shared__ int s_scan[1 + kWholeTries][kDecThreads / 32], s_begin, s_total, s_whole, s_rem, s_at[3], s_stop;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Waits waits{a.err, &s_stop};
   const int group = a.heads / a.cache.kv_heads, chunks = (group + NH - 1) / NH;
   const int subs = a.cache.kv_heads * chunks;
   const int ps = a.cache.page_size, ctas = gridDim.x, cta = blockIdx.x;
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
+    s_stop = 0;
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
           int good = 1;
           if (lane == 0) {
             if (loads >= C::SLOTS)
-              good = mbar_wait(&empty[slot], ph ^ 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
+              good = mbar_wait(&empty[slot], ph ^ 1, waits, tc::ERR_TIMEOUT_PRODUCER);
             if (good) mbar_expect_tx(&full[slot], (uint32_t)(valid * box * HD));
           }
           ok = __shfl_sync(~0u, good, 0);
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     // no copy into this CTA's shared memory may be in flight when it exits
     if (lane == 0)
       for (int i = max(0, loads - C::SLOTS); i < loads; ++i)
-        mbar_wait(&full[i % C::SLOTS], (i / C::SLOTS) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
+        mbar_wait(&full[i % C::SLOTS], (i / C::SLOTS) & 1, waits, tc::ERR_TIMEOUT_PRODUCER, false);
     __syncwarp();
   } else if (warp == 1) {
     // ---- MMA issuer ----
@@ -409,12 +411,12 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     int g = 0, piece = 0;  // tiles and pieces so far
     // tile g of the CTA has its K in load 2g and its V in load 2g + 1
     auto full_of = [&](int load) {
-      return mbar_wait(&full[load % C::SLOTS], (load / C::SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
+      return mbar_wait(&full[load % C::SLOTS], (load / C::SLOTS) & 1, waits, tc::ERR_TIMEOUT_MMA);
     };
     auto qk = [&](int i) -> bool {
       const int slot = (2 * i) % C::SLOTS;
       if (!full_of(2 * i)) return false;
-      if (i >= 2 && !mbar_wait(&s_free[i & 1], ((i >> 1) - 1) & 1, a.err, tc::ERR_TIMEOUT_MMA))
+      if (i >= 2 && !mbar_wait(&s_free[i & 1], ((i >> 1) - 1) & 1, waits, tc::ERR_TIMEOUT_MMA))
         return false;
       tc_fence_after();
       const uint64_t dk = sdesc<ROW>(ring + slot * C::SLOT, 8 * ROW, 0);
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     auto pv = [&](int i, bool first) -> bool {
       const int slot = (2 * i + 1) % C::SLOTS;
       if (!full_of(2 * i + 1) ||
-          !mbar_wait(&p_full[i & 1], (i >> 1) & 1, a.err, tc::ERR_TIMEOUT_MMA))
+          !mbar_wait(&p_full[i & 1], (i >> 1) & 1, waits, tc::ERR_TIMEOUT_MMA))
         return false;
       tc_fence_after();
       // 64-wide heads: both halves of M read the same 64 dimensions (lbo 0)
@@ -456,7 +458,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
       return true;
     };
     while (ok && w.next()) {
-      ok = mbar_wait(&q_full, piece & 1, a.err, tc::ERR_TIMEOUT_MMA) && qk(g);
+      ok = mbar_wait(&q_full, piece & 1, waits, tc::ERR_TIMEOUT_MMA) && qk(g);
       for (int i = 0; i < w.take && ok; ++i, ++g) {
         if (i + 1 < w.take) ok = qk(g + 1);
         ok = ok && pv(g, i == 0);
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
     // every issued MMA completes before TMEM is released
     if (elect_one()) umma_commit(&drain);
     __syncwarp();
-    mbar_wait(&drain, 0, a.err, tc::ERR_TIMEOUT_MMA, false);
+    mbar_wait(&drain, 0, waits, tc::ERR_TIMEOUT_MMA, false);
   } else {
     // ---- softmax and output: warps 2-5 ----
     const int q4 = warp & 3, r = q4 * 32 + lane;
@@ -554,7 +556,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
         const float2 sc1 = scales_of(page1);
         const int page2 = page_of(w.t0 + i + 2);
         const int buf = g & 1;
-        if (ok) ok = mbar_wait(&s_full[buf], (g >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        if (ok) ok = mbar_wait(&s_full[buf], (g >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
         ok = __all_sync(~0u, ok);
         float s[NH];
         if (ok) {
@@ -595,12 +597,12 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
         // P's buffer is free once the P·V of two tiles ago has finished; O may be rescaled once
         // the last one has
         if (ok && g >= 2)
-          ok = mbar_wait(&pv_done[buf], ((g >> 1) - 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+          ok = mbar_wait(&pv_done[buf], ((g >> 1) - 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
         if (i == 0) {
 #pragma unroll
           for (int h = 0; h < NH; ++h) m[h] = top[h];
         } else if (grow) {  // the same for all 128 threads
-          if (ok) ok = mbar_wait(&pv_done[buf ^ 1], ((g - 1) >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+          if (ok) ok = mbar_wait(&pv_done[buf ^ 1], ((g - 1) >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
           ok = __all_sync(~0u, ok);
           float al[NH];
 #pragma unroll
@@ -664,7 +666,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
           // lay in the page or in the ring
           if (__any_sync(~0u, page < 0)) {
             const int load = 2 * g + 1, slot = load % C::SLOTS;
-            ok = mbar_wait(&full[slot], (load / C::SLOTS) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+            ok = mbar_wait(&full[slot], (load / C::SLOTS) & 1, waits, tc::ERR_TIMEOUT_EPI);
             ok = __all_sync(~0u, ok);
             if (ok && page < 0)
 #pragma unroll
@@ -693,7 +695,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
         l[h] = (s_l[0][h] + s_l[1][h]) + (s_l[2][h] + s_l[3][h]);
         inv[h] = 1.f / (16.f * l[h]);
       }
-      if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+      if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
       ok = __all_sync(~0u, ok);
       named_sync<1, 128>();  // s_l may be written again
       const bool whole = w.take == w.nt;

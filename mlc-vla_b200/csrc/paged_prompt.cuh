@@ -248,10 +248,11 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
   __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, q_empty, s_full[2],
       p_full[2][2], pv_done[2], turn[2], drain;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_tiles[C::THREADS], s_scan[WARPS], s_at[4], s_bad;
+  __shared__ int s_tiles[C::THREADS], s_scan[WARPS], s_at[4], s_bad, s_stop;
   __shared__ int64_t s_steps[WARPS], s_begin, s_total;
   __shared__ PromptPiece s_piece[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Waits waits{a.err, &s_stop};
   const int group = a.heads / a.kv_heads, span = NQ * tok;
   const int ctas = gridDim.x, cta = blockIdx.x;
   pdl_trigger();  // every CTA of this grid is resident at once: the joining blocks may queue up
@@ -279,6 +280,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
+    s_stop = 0;
     s_bad = 0x7fffffff;
   }
   if (warp == 1) {
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             const int s = load % SLOTS;
             if (load >= SLOTS)
               ok = ok &&
-                   bar_wait(&empty[s], (load / SLOTS - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
+                   bar_wait(&empty[s], (load / SLOTS - 1) & 1, waits, tc::ERR_TIMEOUT_PRODUCER);
             if (!ok) return nullptr;
             mbar_expect_tx(&full[s], C::SLOT);
             ++load;
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             if (more) load_k(0);
             // the piece before has been begun, and its QKs have read Q
             if (ok && pieces > 0)
-              ok = bar_wait(&q_empty, (pieces - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER);
+              ok = bar_wait(&q_empty, (pieces - 1) & 1, waits, tc::ERR_TIMEOUT_PRODUCER);
             if (!ok) break;
             PromptPiece& pc = s_piece[pieces & 1];
             if (!more) {
@@ -496,9 +498,9 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           }
           // no copy into this CTA's shared memory may be in flight when it exits
           if (ok)
-            bar_wait(&q_full, (pieces - 1) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
+            bar_wait(&q_full, (pieces - 1) & 1, waits, tc::ERR_TIMEOUT_PRODUCER, false);
           for (int l = max(0, load - SLOTS); l < load; ++l)
-            bar_wait(&full[l % SLOTS], (l / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_PRODUCER, false);
+            bar_wait(&full[l % SLOTS], (l / SLOTS) & 1, waits, tc::ERR_TIMEOUT_PRODUCER, false);
         }
         __syncwarp();
       } else if (warp <= NQ) {
@@ -513,7 +515,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         const uint32_t ring = __shfl_sync(~0u, smem_u32(base), 0), tm = __shfl_sync(~0u, tmem, 0);
         const uint32_t qs = ring + SLOTS * C::SLOT + q * C::Q_TILE, to = tm + C::O_COL + q * HD;
         auto full_of = [&](int load) {
-          return bar_wait(&full[load % SLOTS], (load / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_MMA);
+          return bar_wait(&full[load % SLOTS], (load / SLOTS) & 1, waits, tc::ERR_TIMEOUT_MMA);
         };
         auto job_of = [&](int j) { return NQ == 2 ? 2 * (done + j) + q : done + j; };
         auto qk = [&](int j) {
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             if (!ok || !(ok = full_of(load + h))) return;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (!(ok = bar_wait(&p_full[buf][h], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_MMA)))
+            if (!(ok = bar_wait(&p_full[buf][h], (job >> 1) & 1, waits, tc::ERR_TIMEOUT_MMA)))
               return;
             tc_fence_after();
             const int slot = (load + h * (SPT - 1)) % SLOTS;
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           }
         };
         for (;;) {
-          ok = ok && bar_wait(&q_full, pieces & 1, a.err, tc::ERR_TIMEOUT_MMA);
+          ok = ok && bar_wait(&q_full, pieces & 1, waits, tc::ERR_TIMEOUT_MMA);
           if (!ok) break;
           take = s_piece[pieces & 1].take;
           ++pieces;
@@ -589,7 +591,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         // every issued MMA completes before TMEM is released
         if (elect_one()) umma_commit(&drain);
         __syncwarp();
-        bar_wait(&drain, pass, a.err, tc::ERR_TIMEOUT_MMA, false);
+        bar_wait(&drain, pass, waits, tc::ERR_TIMEOUT_MMA, false);
       }
       if (!block_any<C::THREADS>(false)) break;
     }
@@ -606,7 +608,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
       PromptMeta meta{0, 0, 0, 0};
       bool again = false;
       for (;;) {
-        ok = ok && bar_wait(&q_full, pieces & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        ok = ok && bar_wait(&q_full, pieces & 1, waits, tc::ERR_TIMEOUT_EPI);
         // in the second pass the warpgroups meet below: there one's failure is the other's
         ok = pass == 1 ? softmax_all<NQ>(ok) : softmax_all<1>(ok, 2 + wg);
         if (!ok) break;
@@ -627,7 +629,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           constexpr bool careful = decltype(second)::value;
           const int job = NQ == 2 ? 2 * (done + t) + wg : done + t, buf = job & 1;
           const int key0 = pc.key0 + t * kKeys;
-          if (ok) ok = bar_wait(&s_full[buf], (job >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+          if (ok) ok = bar_wait(&s_full[buf], (job >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
           ok = __all_sync(~0u, ok);
           if (ok) {
             tc_fence_after();
@@ -648,7 +650,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             } else if (__any_sync(~0u, top > m + kPromptGrow)) {
               // the sums so far are complete once the P·V before has finished
               const int prev = NQ == 2 ? job - 2 : job - 1;
-              ok = bar_wait(&pv_done[prev & 1], (prev >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+              ok = bar_wait(&pv_done[prev & 1], (prev >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
               ok = __all_sync(~0u, ok);
               if (ok) {
                 float al = 1.f;
@@ -672,7 +674,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             // The exponentials of the two warpgroups take turns: at the same time they would hold
             // each other up, and then both leave the tensor cores without work.
             if constexpr (NQ == 2)
-              ok = bar_wait(&turn[wg], (done + t) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+              ok = bar_wait(&turn[wg], (done + t) & 1, waits, tc::ERR_TIMEOUT_EPI);
             const float ref = m == -INFINITY ? 0.f : m;
             const uint64_t c2 = pack2(c, c), r2 = pack2(-ref, -ref);
             uint64_t sum0 = 0, sum1 = 0;  // two zeros each
@@ -711,7 +713,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
 #pragma unroll 1
             for (int h = 0; h < SPT; ++h) {
               const int sl = (load + h) % SLOTS;
-              if (ok) ok = bar_wait(&full[sl], ((load + h) / SLOTS) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+              if (ok) ok = bar_wait(&full[sl], ((load + h) / SLOTS) & 1, waits, tc::ERR_TIMEOUT_EPI);
               ok = __all_sync(~0u, ok);
               if (!ok) break;
 #pragma unroll 1
@@ -752,7 +754,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         const bool whole = pc.slot < 0;
         const int64_t row_at = (int64_t)(pc.q0 + i) * a.o_tok +
                                (int64_t)(pc.kv * group + r % group) * a.o_head;
-        if (ok) ok = bar_wait(&pv_done[last & 1], (last >> 1) & 1, a.err, tc::ERR_TIMEOUT_EPI);
+        if (ok) ok = bar_wait(&pv_done[last & 1], (last >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
         ok = __all_sync(~0u, ok);
         tc_fence_after();
         int bad = 0x7fffffff;

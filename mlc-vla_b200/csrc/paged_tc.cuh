@@ -11,7 +11,6 @@ using tc::globaltimer;
 using tc::mbar_arrive;
 using tc::mbar_expect_tx;
 using tc::mbar_init;
-using tc::mbar_wait;
 using tc::tc_fence_after;
 using tc::tc_fence_before;
 using tc::tma_prefetch_desc;
@@ -141,22 +140,42 @@ __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// tc::mbar_wait without its call, for kernels that shift registers between warps (setmaxnreg allows
-// no call)
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* err, int code,
-                                         bool bail = true) {
-  if (tc::mbar_try(bar, parity)) return true;
+// Bounded waits of one CTA (about a second of globaltimer each). One that gives up records its code
+// for the call and sets the CTA's `stop`, at which its other waits give up as well. They do not look
+// at *err: it may hold what an earlier call or another request has recorded.
+struct Waits {
+  int* err;
+  volatile int* stop;  // shared memory, zero at the start
+};
+__device__ __forceinline__ bool wait_polling(uint64_t* bar, uint32_t parity, const Waits& w, int code,
+                                             bool bail) {
   const unsigned long long t0 = globaltimer();
   for (uint32_t it = 1;; ++it) {
     if (tc::mbar_try(bar, parity)) return true;
     if ((it & 127) == 0) {
+      if (bail && *w.stop) return false;
       if (globaltimer() - t0 > tc::kTimeoutNs) {
-        atomicCAS(err, 0, code);
+        atomicCAS(w.err, 0, code);
+        *w.stop = 1;
         return false;
       }
-      if (bail && (it & 8191) == 0 && *(volatile int*)err != 0) return false;
     }
   }
+}
+static __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, Waits w, int code,
+                                              bool bail) {
+  return wait_polling(bar, parity, w, code, bail);
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const Waits& w, int code,
+                                          bool bail = true) {
+  if (tc::mbar_try(bar, parity)) return true;
+  return wait_slow(bar, parity, w, code, bail);
+}
+// the same without a call, for kernels that shift registers between warps (setmaxnreg allows none)
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, const Waits& w, int code,
+                                         bool bail = true) {
+  if (tc::mbar_try(bar, parity)) return true;
+  return wait_polling(bar, parity, w, code, bail);
 }
 
 // One thread of a converged warp. Tensor-core instructions are issued by a whole warp's control flow

@@ -227,3 +227,79 @@ def test_paged_batch_without_any_token(batch, heads, kv_heads, dim, page):
     paged.attention_paged(q, c, table, dev(lens), out=out)
     paged.check()
     assert not out[:-1].any() and (out[-1] == 0.5).all()
+
+
+# ---- attention over prompts, and both ---------------------------------------------------------------
+
+def filled_cache(rng, lens, page, heads, dim):
+    """A cache of random codes in which requests hold `lens` tokens, with its table."""
+    from mlc_vla import paged
+
+    counts = [-(-n // page) for n in lens]
+    order = rng.permutation(sum(counts) + 2)
+    table, at = np.full((len(lens), max(counts)), -1), 0
+    for r, n in enumerate(counts):
+        table[r, :n] = order[at:at + n]
+        at += n
+    codes = [rng.integers(0, 256, (len(order), heads, page, dim)).astype(np.uint8) for _ in range(2)]
+    for x in codes:
+        x[(x & 0x7F) == 0x7F] = 0
+    return paged.KVCache8(*(torch.as_tensor(x).cuda().view(torch.float8_e4m3fn) for x in codes),
+                          *(torch.full((len(order), heads), 2.0 ** -7, device="cuda")
+                            for _ in range(2))), table
+
+
+@pytest.mark.parametrize("code", [1, 18, 1000])
+def test_a_recorded_error_does_not_reach_later_calls(code):
+    """`err` keeps the first code; waits that take long must not give up at one that is there already."""
+    from mlc_vla import paged
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def rows(*shape):
+        return torch.randn(shape, generator=g, device="cuda").half()
+
+    new, held = [300, 20, 700], [3800, 10, 0]
+    cu_q, cu_k = dev(np.cumsum([0] + new)), dev(np.cumsum([0] + [a + b for a, b in zip(new, held)]))
+    rng = np.random.default_rng(0)
+    for heads, kv_heads, dim in ((4, 2, 128), (8, 1, 256), (2, 2, 64)):
+        q, k, v = rows(1020, heads, dim), rows(4830, kv_heads, dim), rows(4830, kv_heads, dim)
+        odd = v.clone()
+        odd[4099, :, 5] = float("inf")  # the last key of the first request, seen by its last query
+        lens = [3000, 5, 900, 129]
+        c, table = filled_cache(rng, lens, 16, kv_heads, dim)
+        qd = rows(4, heads, dim)
+        for values in (v, odd):
+            got = []
+            for first in (0, code):
+                err = dev([first])
+                got.append((paged.attention_prompt(q, k, values, cu_q, cu_k, err=err),
+                            paged.attention_paged(qd, c, dev(table), dev(lens), err=err)))
+                assert int(err.item()) == first
+            for a, b in zip(*got):
+                assert torch.equal(a.nan_to_num(), b.nan_to_num())
+                assert torch.equal(a.isnan(), b.isnan())
+            clean = torch.isfinite(got[1][0])
+            if values is odd:
+                assert not clean[299, :, 5].any()
+                clean[299, :, 5] = True
+            assert clean.all() and torch.isfinite(got[1][1]).all()
+
+
+@pytest.mark.parametrize("dim,page", [(128, 16), (256, 64), (64, 8)])
+def test_a_bad_page_does_not_reach_other_requests(dim, page):
+    from mlc_vla import paged
+
+    rng = np.random.default_rng(dim)
+    lens = [2000, 700, 1, 4000, 333] * 4
+    c, table = filled_cache(rng, lens, page, 1, dim)
+    q = torch.as_tensor(rng.standard_normal((20, 8, dim))).half().cuda()
+    clean = paged.attention_paged(q, c, dev(table), dev(lens))
+    paged.check()
+    bad = table.copy()
+    bad[3, 5], bad[8, 0] = len(c.k), -1
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = paged.attention_paged(q, c, dev(bad), dev(lens), err=err)
+    assert int(err.item()) == 19
+    good = [r for r in range(20) if r not in (3, 8)]
+    assert torch.equal(out[good], clean[good])
