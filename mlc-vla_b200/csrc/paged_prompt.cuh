@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
   __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], q_full, q_empty, s_full[2],
       p_full[2][2], pv_done[2], turn[2], drain;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_tiles[C::THREADS], s_scan[WARPS], s_at[4], s_bad, s_stop;
+  __shared__ int s_tiles[C::THREADS], s_scan[WARPS], s_at[4], s_stop;
+  __shared__ uint32_t s_odd[kKeys / 32];  // keys of a tile whose values are no numbers
   __shared__ int64_t s_steps[WARPS], s_begin, s_total;
   __shared__ PromptPiece s_piece[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -281,7 +282,6 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
     s_stop = 0;
-    s_bad = 0x7fffffff;
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
 
   // A row whose sum meets an infinity or a NaN may owe it to a value that it does not see (weight
   // zero times infinity): then the CTA does its share once more, with such values taken out of the
-  // V tiles that some rows of a piece see in part.
+  // V tiles that some rows of a piece see in part, and added to the sums of the rows that see them.
   // A row of 128 logits takes more registers than 1/12 of an SM's: where there are twelve warps, the
   // first warpgroup gives some of its own. (80 + 2·208)·128 of the 168·384 that the block was
   // launched with.
@@ -706,9 +706,12 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
             if (!careful && lane == 0) mbar_arrive(&p_full[buf][1]);  // the other tile can wait, P·V not
             if (NQ == 2 && lane == 0) mbar_arrive(&turn[wg ^ 1]);
           }
-          if (careful && key0 + kKeys > pc.fewest) {
-            // V rows of this tile, by all softmax warps: values that are no numbers become zero;
-            // s_bad keeps the first key of the request that lost one
+          const bool in_part = careful && key0 + kKeys > pc.fewest;  // the same for all rows
+          if (in_part) {
+            // V rows of this tile, by all softmax warps: values that are no numbers become zero
+            named_sync<1, NQ * 128>();  // s_odd of the step before has been read
+            if (tid - 128 < kKeys / 32) s_odd[tid - 128] = 0;
+            named_sync<1, NQ * 128>();
             const int load = (2 * done + v_unit(t, take)) * SPT;
 #pragma unroll 1
             for (int h = 0; h < SPT; ++h) {
@@ -718,7 +721,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
               if (!ok) break;
 #pragma unroll 1
               for (int v = tid - 128; v < C::SLOT / 16; v += NQ * 128) {
-                const int key = key0 + h * C::VKEYS + (v / 8) % C::VKEYS;
+                const int key = h * C::VKEYS + (v / 8) % C::VKEYS;  // within the tile
                 uint4* at = reinterpret_cast<uint4*>(base + sl * C::SLOT) + v;
                 uint4 x4 = *at;
                 T* e = reinterpret_cast<T*>(&x4);
@@ -731,7 +734,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
                   }
                 if (hit) {
                   *at = x4;
-                  if (key < pc.lk) atomicMin(&s_bad, key);
+                  if (key0 + key < pc.lk) atomicOr(&s_odd[key / 32], 1u << (key % 32));
                 }
               }
             }
@@ -742,6 +745,39 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
           if (careful && ok && lane == 0) {  // only now is V what it should be
             mbar_arrive(&p_full[buf][0]);
             mbar_arrive(&p_full[buf][1]);
+          }
+          if (in_part && (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3])) {
+            // what was taken out reaches the rows that see it as it is: any weight of an infinity is one
+            if (ok) ok = bar_wait(&pv_done[buf], (job >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
+            ok = __all_sync(~0u, ok);
+            if (ok) {
+              tc_fence_after();
+              const T* v0 = reinterpret_cast<const T*>(a.v) + (int64_t)(pc.k0 + key0) * a.v_tok +
+                            pc.kv * a.v_head;
+#pragma unroll 1
+              for (int d = 0; d < HD; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(tO + d, o);
+#pragma unroll 1
+                for (int j = 0; j < kKeys; ++j) {
+                  if (!(s_odd[j / 32] >> (j % 32) & 1)) continue;
+                  const bool sees = key0 + j < mine;
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) {
+                    float x[8];
+                    load8(v0 + j * a.v_tok + d + c * 8, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                      if (sees && !isfinite(x[e]))
+                        o[c * 8 + e] = __float_as_uint(__uint_as_float(o[c * 8 + e]) + x[e]);
+                  }
+                }
+                __syncwarp();
+                tmem_st32(tO + d, o);
+              }
+              tmem_wait_st();
+              tc_fence_before();
+            }
           }
         };
         if (pass == 0) {
@@ -757,14 +793,6 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         if (ok) ok = bar_wait(&pv_done[last & 1], (last >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
         ok = __all_sync(~0u, ok);
         tc_fence_after();
-        int bad = 0x7fffffff;
-        if (pass == 1) {
-          named_sync<1, NQ * 128>();  // s_bad is final for this piece
-          bad = s_bad;
-          named_sync<1, NQ * 128>();
-          if (tid == 128) s_bad = 0x7fffffff;
-          named_sync<1, NQ * 128>();
-        }
         // o = O / l, or O as it is for the joining kernel. A row that sees no key is zero, and one of
         // a kernel that gave up waiting NaN.
         const float inv = !ok ? NAN : whole ? 1.f / l : 1.f;
@@ -842,39 +870,13 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         const float2 nan = unpack2(add2(nan2[0], nan2[1]));
         const bool odd = row && mine > 0 && ok && !(nan.x + nan.y == 0.f);
         again |= odd;
-        // rows that do see a value that was taken out, unless nothing in them is a number anyway
-        bool fix = false;
-        if (pass == 1 && __any_sync(~0u, mine > bad)) {
-          bool all = true;
-#pragma unroll 1
-          for (int d = 0; d < HD; d += 32) {
-            uint32_t o[32];
-            tmem_ld32(tO + d, o);
-#pragma unroll
-            for (int u = 0; u < 32; ++u) all &= !isfinite(__uint_as_float(o[u]));
-          }
-          fix = row && ok && mine > bad && !all;
-        }
         tc_fence_before();
         if (!whole) {
           float* ml = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + pc.slot) * C::PARTIAL +
                       wg * C::PART_TILE + 128 * HD;
           ml[r] = m;
-          ml[128 + r] = fix ? -1.f : l;  // no sum is negative: a sign for the joining kernel
+          ml[128 + r] = l;
           if (pc.count > 0) meta = PromptMeta{pc.request, pc.tile, pc.kv, pc.count};
-        } else if (pass == 1) {
-          unsigned redo = __ballot_sync(~0u, fix);
-          while (redo) {
-            const int rr = q4 * 32 + __ffs(redo) - 1, ii = tq + rr / group;
-            redo &= redo - 1;
-            const int64_t hh = pc.kv * group + rr % group;
-            const PromptKV<T> src{
-                reinterpret_cast<const T*>(a.k) + pc.k0 * a.k_tok + pc.kv * a.k_head,
-                reinterpret_cast<const T*>(a.v) + pc.k0 * a.v_tok + pc.kv * a.v_head, a.k_tok, a.v_tok};
-            attend_row(reinterpret_cast<const T*>(a.q) + (pc.q0 + ii) * a.q_tok + hh * a.q_head, HD,
-                       visible(ii, pc.lq, pc.lk, pc.prefix), a.c, src,
-                       reinterpret_cast<T*>(a.out) + (pc.q0 + ii) * a.o_tok + hh * a.o_head);
-          }
         }
       }
       if (tid == 128) reinterpret_cast<PromptMeta*>(a.ws)[cta] = meta;
@@ -906,7 +908,6 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a, int tok,
   const float* first = a.ws + (size_t)ctas * 4 + ((size_t)cta * 2 + 1) * C::PARTIAL +
                        wg * C::PART_TILE;
   float M = -INFINITY, l = 0.f, o[32];
-  bool fix = false;
 #pragma unroll
   for (int u = 0; u < 32; ++u) o[u] = 0.f;
   for (int p = 0; p < meta.count; ++p) {
@@ -917,7 +918,6 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a, int tok,
 #pragma unroll
     for (int u = 0; u < 8; ++u)
       v[u] = *reinterpret_cast<const float4*>(part + ((size_t)(d0 / 4 + u) * 128 + r) * 4);
-    fix |= pl < 0.f;
     const float top = fmaxf(M, pm), ref = top == -INFINITY ? 0.f : top;
     const float old = exp2f(M - ref), f = exp2f(pm - ref);
     M = top;
@@ -931,7 +931,7 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a, int tok,
     }
   }
   const int64_t h = meta.kv * group + r % group;
-  if (row && !fix) {
+  if (row) {
     const float inv = 1.f / l;
     const uint32_t keep = seq.sees(i) > 0 ? ~0u : 0u;  // a row that sees no key is zero
     T* out = reinterpret_cast<T*>(a.out) + (int64_t)(seq.q0 + i) * a.o_tok + h * a.o_head + d0;
@@ -943,18 +943,6 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a, int tok,
       for (int e = 0; e < 4; ++e) pw[e] = Tr<T>::pack(o[u + 2 * e] * inv, o[u + 2 * e + 1] * inv) & keep;
       *reinterpret_cast<uint4*>(out + u) = pk;
     }
-  }
-  unsigned redo = d0 == 0 ? __ballot_sync(~0u, row && fix) : 0u;
-  while (redo) {
-    const int rr = (r & ~31) + __ffs(redo) - 1, ii = tq + rr / group;
-    redo &= redo - 1;
-    const int64_t hh = meta.kv * group + rr % group;
-    const PromptKV<T> src{reinterpret_cast<const T*>(a.k) + seq.k0 * a.k_tok + meta.kv * a.k_head,
-                          reinterpret_cast<const T*>(a.v) + seq.k0 * a.v_tok + meta.kv * a.v_head,
-                          a.k_tok, a.v_tok};
-    attend_row(reinterpret_cast<const T*>(a.q) + (seq.q0 + ii) * a.q_tok + hh * a.q_head, HD,
-               seq.sees(ii), a.c, src,
-               reinterpret_cast<T*>(a.out) + (seq.q0 + ii) * a.o_tok + hh * a.o_head);
   }
 }
 

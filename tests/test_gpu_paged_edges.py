@@ -303,3 +303,54 @@ def test_a_bad_page_does_not_reach_other_requests(dim, page):
     assert int(err.item()) == 19
     good = [r for r in range(20) if r not in (3, 8)]
     assert torch.equal(out[good], clean[good])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(8, 1, 256, "float16"), (4, 2, 128, "bfloat16"),
+                                                      (16, 1, 64, "float16"), (3, 3, 128, "float16")])
+@pytest.mark.parametrize("new,held,prefix", [
+    ([200], [69900], None), ([1500, 3, 260], [0, 20000, 4100], None), ([900, 700], [0, 0], [400, 768]),
+    ([100], [5], None)])
+def test_values_that_are_no_numbers_reach_their_rows_only(heads, kv_heads, dim, dtype, new, held, prefix):
+    """Where some rows of a tile see such a value and others do not: the others, and the other
+    dimensions, keep their bits, however long the request is."""
+    from mlc_vla import paged
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    cu_q, cu_k = np.cumsum([0] + new), np.cumsum([0] + [a + b for a, b in zip(new, held)])
+
+    def rows(n, h):
+        return torch.randn((n, h, dim), generator=g, device="cuda").to(getattr(torch, dtype))
+
+    q, k, v = rows(cu_q[-1], heads), rows(cu_k[-1], kv_heads), rows(cu_k[-1], kv_heads)
+
+    def attend(values):
+        out = paged.attention_prompt(q, k, values, dev(cu_q), dev(cu_k),
+                                     prefix_lens=None if prefix is None else dev(prefix))
+        paged.check()
+        return out
+
+    clean, inf = attend(v), float("inf")
+    assert torch.isfinite(clean).all()
+    odd = v.clone()
+    marks = []  # request, key, dimension, value
+    for r, (n, h) in enumerate(zip(new, held)):
+        marks += [(r, h + j, d, x) for j, d, x in ((n - 1, 0, inf), (n // 2, 5, -inf), (n // 3, 33, inf),
+                                                   (2 * n // 3, 33, -inf), (n // 2, dim - 1, inf - inf))]
+    marks.append((0, 0, 40, -inf))  # seen by every row of the first request
+    for r, j, d, x in marks:
+        odd[cu_k[r] + j, :, d] = x
+    got, want = attend(odd), clean.float()
+    for r, n in enumerate(new):
+        lk = n + held[r]
+        sees = torch.arange(n, device="cuda") + held[r] + 1
+        if prefix is not None:
+            sees = sees.clamp_min(prefix[r]).clamp_max(lk)
+        for m, j, d, x in marks:
+            if m == r:
+                want[cu_q[r]:cu_q[r + 1], :, d] += torch.where(sees > j, x, 0.0)[:, None]
+    finite = torch.isfinite(want)
+    assert torch.equal(got[finite], clean[finite])
+    # an infinity whose weight is no longer a number above zero gives NaN
+    rest = got[~finite].float()
+    assert ((rest == want[~finite]) | rest.isnan()).all()
+    assert (rest.isnan() | ~want[~finite].isnan()).all()
