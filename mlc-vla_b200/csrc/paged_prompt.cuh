@@ -110,7 +110,14 @@ __global__ void __launch_bounds__(32 * kRowWarps) prompt_rows_kernel(PromptArgs 
 // ---- tensor-core form -----------------------------------------------------------------------------
 
 constexpr int kKeys = 128;             // keys per tile
-constexpr float kPromptGrow = 8.f;     // the reference maximum is raised when it would grow by 2^8
+constexpr float kPromptGrow = 8.f;     // the reference is raised when the maximum has outgrown it by 2^8
+
+// How far the reference lies below the maximum that it is taken from. Weights are held in the type of V:
+// in fp16, those below 2^-14 lose bits and those below 2^-25 are zero, while the fp32 sum counts them.
+// Lifted by 2^7 they reach 2^15 at most, with what the maximum may outgrow, and keep their bits down
+// to 2^-21 of the largest. bf16 has fp32's range.
+template <typename T>
+constexpr float kLift = Tr<T>::kBf16 ? 0.f : 7.f;
 
 template <int HD>
 struct PromptCfg {
@@ -644,7 +651,7 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
 #pragma unroll
               for (int u = 0; u < 128; ++u) s[u] = u < lim ? s[u] : -INFINITY;
             }
-            const float top = max128(s) * c;
+            const float top = max128(s) * c - kLift<T>;
             if (t == 0) {
               m = top;
             } else if (__any_sync(~0u, top > m + kPromptGrow)) {

@@ -354,3 +354,51 @@ def test_values_that_are_no_numbers_reach_their_rows_only(heads, kv_heads, dim, 
     rest = got[~finite].float()
     assert ((rest == want[~finite]) | rest.isnan()).all()
     assert (rest.isnan() | ~want[~finite].isnan()).all()
+
+
+# ---- small weights --------------------------------------------------------------------------------
+
+def sink_error(out, q, k, v, dtype, step):
+    """Largest error, in parts of its bound, of rows [queries, dim] that see all keys: rounding of the
+    result and of the weights (u each, and of their sum), fp32 logits (2^-23 of each product; 2^-21 of
+    the logit and 2^-20 for the exponential, in numerator and denominator), the fp32 sum; and `step`,
+    what a weight below the normal range of its form loses at most, in units of the row's largest."""
+    q, k, v = q.double(), k.double(), v.double()
+    n, dim = k.shape
+    s = q @ k.T * dim ** -0.5
+    p = torch.softmax(s, -1)
+    o, spread = p @ v, p @ v.abs()
+    size = (q.abs() @ k.abs().T).amax(1, True) * dim ** -0.5
+    u = {"float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}[dtype]
+    logit = 2 * (dim * 2.0 ** -23 * size + 2.0 ** -21 * s.abs().amax(1, True) + 2.0 ** -20)
+    tol = (u * o.abs() + (2 * u + logit + n * 2.0 ** -23) * spread + n * step * v.abs().max()
+           + 2.0 ** -25)  # half a step of fp16's results below its normal range
+    return float(((out.double() - o).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("heads,dim,new", [(64, 256, 150), (32, 128, 600), (16, 64, 1200)])
+@pytest.mark.parametrize("gap", [15, 20, 23, 25])
+def test_prompt_one_key_above_all_others(heads, dim, new, dtype, gap):
+    """A first key `gap` bits above the rest whose value is zero: the result is what thousands of
+    small weights add up to. In fp16 weights are held in steps of 2^-24 below 2^-14, lifted by 2^7.
+    Requests enough that a CTA takes all keys of some tiles."""
+    from mlc_vla import paged
+
+    g = torch.Generator(device="cuda").manual_seed(gap + dim)
+    batch, n, kv_heads = 4, 4200, 8
+    q = torch.randn((batch * new, heads, dim), generator=g, device="cuda")
+    k = torch.randn((batch * n, kv_heads, dim), generator=g, device="cuda") * 0.5
+    v = 1.0 + 0.1 * torch.randn((batch * n, kv_heads, dim), generator=g, device="cuda")
+    q[:, :, 0], k[:, :, 0], k[::n], v[::n] = 8.0, 0.0, 0.0, 0.0
+    k[::n, :, 0] = gap * np.log(2.0) * dim ** 0.5 / 8.0
+    q, k, v = (x.to(getattr(torch, dtype)) for x in (q, k, v))
+    out = paged.attention_prompt(q, k, v, dev(np.arange(batch + 1) * new), dev(np.arange(batch + 1) * n),
+                                 prefix_lens=dev([n] * batch))
+    paged.check()
+    step = 2.0 ** -32 if dtype == "float16" else 0.0
+    for r in range(batch):
+        rows, keys = slice(r * new, (r + 1) * new), slice(r * n, (r + 1) * n)
+        worst = max(sink_error(out[rows, h], q[rows, h], k[keys, h // (heads // kv_heads)],
+                               v[keys, h // (heads // kv_heads)], dtype, step) for h in range(heads))
+        assert worst <= 1.0, worst
