@@ -10,11 +10,14 @@
 //     added in fp32.
 //   * weights: w = exp2(s − M) in fp32 with s = c·ks·Σ…, their sum l in fp32. V needs the weight
 //     times its page's scale, so the reference M is the running maximum of s + log2 vs: then
-//     p = 16·w·vs ≤ 16 whatever the scales are. M is only raised, and the sums rescaled, when it
-//     would grow by more than 2^4, so p ≤ 256 fits e4m3 (448).
-//   * values:  Oᵀ += Vᵀ·Pᵀ, M = 128 dimensions, p as three e4m3 parts again: 12 bits of each
-//     weight, one more than fp16 has, down to 2^-22 of the largest.
-//   * o = Oᵀ/(16·l).
+//     p = 256·w·vs ≤ 256 whatever the scales are. M is only raised, and the sums rescaled, when it
+//     would grow by more than 2^0.8, so p ≤ 446 fits e4m3 (448).
+//   * values:  Oᵀ += Vᵀ·Pᵀ, M = 128 dimensions, p as four e4m3 parts, p₁ + p₂/16 + p₃/256 + p₄/4096:
+//     16 bits of each weight, in steps of 2^-21: what a weight loses is at most 2^-30 of the largest
+//     w·vs. (A page louder than the others counts with its scale, whatever its tokens' weights are.)
+//     Three parts of p ≤ 16 in the same columns lost what lay below 2^-22 of the largest, a third of
+//     the result where one key of value zero stood 23 bits above 16384 others.
+//   * o = Oᵀ/(256·l).
 //
 // Bound by HBM: 2 bytes per key, kv head and dimension. Per tile of 128 keys and 256 dimensions
 // (64 KB, 1.5 µs of one SM's share of HBM) the MMAs are 16 instructions of N = 32 and the softmax
@@ -115,7 +118,8 @@ constexpr int kDecTile = 128;          // keys per tile
 constexpr int kDecThreads = 192;
 constexpr int kWholeTiles = 8;         // pieces of up to so many tiles keep to one unit
 constexpr int kWholeTries = 4;         // lengths tried: the least that could do, and some more
-constexpr float kDecGrow = 4.f;        // M is raised when it would grow by more than 2^4
+constexpr float kDecTop = 256.f;       // the weight at M, as it enters the product
+constexpr float kDecGrow = 0.8f;       // M is raised when it would grow by more than 2^0.8
 
 template <int HD, int NH>
 struct DecCfg {
@@ -123,7 +127,7 @@ struct DecCfg {
   static constexpr int HB = (HD + 127) / 128;       // 128-wide blocks of the head dimension
   static constexpr int SLOT = kDecTile * HD;        // a K or a V tile
   static constexpr int BLOCK = kDecTile * ROW;      // one 128-wide block of it
-  // columns: three parts × heads, then empty ones; COLS of them are read back
+  // columns: parts × heads (the fourth of q is empty), then empty ones; COLS of them are read back
   static constexpr int N = NH < 8 ? 32 : 4 * NH;
   static constexpr int COLS = 4 * NH;
   static constexpr int Q_BYTES = N * HD;
@@ -192,11 +196,13 @@ __device__ __forceinline__ float on_e4m3(float x) {
   return __fsub_rn(__fadd_rn(x, big), big);
 }
 
-// x = p₁ + p₂/16 + p₃/256, each an e4m3 code: the codes of two values for each part
-__device__ __forceinline__ void split3(float x, float y, uint32_t (&part)[3]) {
+// x = p₁ + p₂/16 + p₃/256 …, each an e4m3 code: the codes of two values for each part
+template <int PARTS>
+__device__ __forceinline__ void split(float x, float y, uint32_t (&part)[PARTS]) {
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < PARTS; ++i) {
     part[i] = e4m3x2(x, y);
+    if (i + 1 == PARTS) break;
     x = (x - on_e4m3(x)) * 16.f;
     y = (y - on_e4m3(y)) * 16.f;
   }
@@ -513,7 +519,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
           uint32_t part[3];
           // an infinite entry has no code and makes the whole row NaN, as every logit would be
           const float y0 = isinf(v[e]) ? NAN : v[e] * inv, y1 = isinf(v[e + 1]) ? NAN : v[e + 1] * inv;
-          split3(y0, y1, part);
+          split(y0, y1, part);
 #pragma unroll
           for (int p = 0; p < 3; ++p) codes[p][e / 2] = (uint16_t)part[p];
         }
@@ -631,8 +637,8 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
           }
         }
         ok = __all_sync(~0u, ok);
-        // weights, in three parts each, as this key's row of P: N consecutive bytes
-        uint32_t word[3][NH / 4];
+        // weights, in four parts each, as this key's row of P: N consecutive bytes
+        uint32_t word[4][NH / 4];
 #pragma unroll
         for (int h = 0; h < NH; h += 2) {
           const float r0 = m[h] == -INFINITY ? 0.f : m[h];
@@ -640,11 +646,11 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
           const float e0 = exp2_fast(s[h] - r0), e1 = exp2_fast(s[h + 1] - r1);
           l[h] += e0;
           l[h + 1] += e1;
-          uint32_t part[3];
-          const float f = 16.f * sc.y;
-          split3(e0 * f, e1 * f, part);
+          uint32_t part[4];
+          const float f = kDecTop * sc.y;
+          split(e0 * f, e1 * f, part);
 #pragma unroll
-          for (int p = 0; p < 3; ++p) {
+          for (int p = 0; p < 4; ++p) {
             if (h % 4 == 0) word[p][h / 4] = part[p];
             else word[p][h / 4] |= part[p] << 16;
           }
@@ -658,7 +664,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int n = n0 + 4 * j;
-              qw[j] = n / NH < 3 ? word[n / NH < 3 ? n / NH : 0][(n % NH) / 4] : 0u;
+              qw[j] = word[n / NH][(n % NH) / 4];
             }
             *reinterpret_cast<uint4*>(p + swz<N>(r * N + n0)) = q;
           }
@@ -693,7 +699,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         l[h] = (s_l[0][h] + s_l[1][h]) + (s_l[2][h] + s_l[3][h]);
-        inv[h] = 1.f / (16.f * l[h]);
+        inv[h] = 1.f / (kDecTop * l[h]);
       }
       if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
       ok = __all_sync(~0u, ok);
@@ -715,6 +721,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
             if (p == 0) o[h] = f;
             else if (p == 1) o[h] = fmaf(f, 1.f / 16.f, o[h]);
             else if (p == 2) o[h] = fmaf(f, 1.f / 256.f, o[h]);
+            else o[h] = fmaf(f, 1.f / 4096.f, o[h]);
           }
         }
         const int d = hb * 128 + r;
@@ -758,7 +765,7 @@ __global__ void __launch_bounds__(kDecThreads, DecCfg<HD, NH>::OCC)
 }
 
 // Joins the partials of the unit that begins in CTA blockIdx.x and ends in another: one block per
-// (CTA, head), out = Σ 2^(Mᵢ−M)·oᵢ / (16·Σ 2^(Mᵢ−M)·lᵢ). A thread takes one dimension of every JS-th
+// (CTA, head), out = Σ 2^(Mᵢ−M)·oᵢ / (256·Σ 2^(Mᵢ−M)·lᵢ). A thread takes one dimension of every JS-th
 // eight partials, whose loads are in flight together; the JS sums are joined in order.
 constexpr int kJoinThreads = 512;
 
@@ -820,7 +827,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(DecodeArgs a, 
   }
   if (js == 0)
     reinterpret_cast<T*>(a.out)[meta.batch * a.o_tok + (meta.head + h) * a.o_head + d] =
-        Tr<T>::t(o / (16.f * l));
+        Tr<T>::t(o / (kDecTop * l));
 }
 
 }  // namespace paged

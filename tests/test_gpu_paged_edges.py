@@ -402,3 +402,75 @@ def test_prompt_one_key_above_all_others(heads, dim, new, dtype, gap):
         worst = max(sink_error(out[rows, h], q[rows, h], k[keys, h // (heads // kv_heads)],
                                v[keys, h // (heads // kv_heads)], dtype, step) for h in range(heads))
         assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,batch", [
+    (8, 1, 256, 64, 320), (4, 1, 128, 16, 640), (8, 1, 64, 8, 640), (3, 1, 64, 128, 900),
+    (16, 1, 128, 32, 320), (12, 1, 256, 16, 200)])
+@pytest.mark.parametrize("gap", [18, 22, 23, 25])
+def test_paged_one_key_above_all_others(heads, kv_heads, dim, page, batch, gap):
+    """The same over the cache, where weights are held as sums of e4m3 parts, in steps of 2^-29 of the
+    largest (half of that is lost at most). Many requests on the same pages, so that a CTA takes all
+    keys of some of them. Values of page 0, the sink's, are zero."""
+    from mlc_vla import paged
+
+    g = torch.Generator(device="cuda").manual_seed(gap + dim)
+    n, pages = 16384 + 5, -(-(16384 + 5) // page)
+    k = (4.0 * torch.randn((pages, 1, page, dim), generator=g, device="cuda")).to(torch.float8_e4m3fn)
+    v = torch.randint(0x58, 0x60, (pages, 1, page, dim), generator=g, device="cuda",
+                      dtype=torch.uint8).view(torch.float8_e4m3fn)  # 16 to 30
+    k.view(torch.uint8)[..., 0] = 0
+    k.view(torch.uint8)[0, 0, 0] = 0
+    v.view(torch.uint8)[0, 0, 0] = 0
+    k[0, 0, 0, 0] = 256.0
+    k_scale = torch.full((pages, 1), 2.0 ** -3, device="cuda")
+    v_scale = torch.full((pages, 1), 2.0 ** -5, device="cuda")
+    q = torch.randn((batch, heads, dim), generator=g, device="cuda")
+    q[:, :, 0] = gap * np.log(2.0) * dim ** 0.5 / 32.0
+    q = q.half()
+    c = paged.KVCache8(k, v, k_scale, v_scale)
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).expand(batch, pages).contiguous()
+    out = paged.attention_paged(q, c, table, dev([n] * batch))
+    paged.check()
+    kn, vn = (x.double().reshape(-1, dim)[:n] * s for x, s in ((k, 2.0 ** -3), (v, 2.0 ** -5)))
+    rows, got = q.reshape(-1, dim), out.reshape(-1, dim)
+    for a in range(0, len(rows), 640):
+        worst = sink_error(got[a:a + 640], rows[a:a + 640], kn, vn, "float16", 2.0 ** -30)
+        assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("heads,dim,page", [(8, 256, 64), (4, 128, 16), (16, 64, 32)])
+@pytest.mark.parametrize("loud", [8, 14])
+def test_paged_loud_page(heads, dim, page, loud):
+    """A page whose scale is 2^`loud` above the others, because of one token of no weight: the weights
+    of the others are taken relative to the page's scale and have as many bits less."""
+    from mlc_vla import paged
+
+    g = torch.Generator(device="cuda").manual_seed(loud + dim)
+    batch, n = 640, 2048
+    pages = n // page
+    k = (8.0 * torch.randn((pages, 1, page, dim), generator=g, device="cuda")).to(torch.float8_e4m3fn)
+    v = torch.randint(0x58, 0x60, (pages, 1, page, dim), generator=g, device="cuda",
+                      dtype=torch.uint8).view(torch.float8_e4m3fn)
+    k.view(torch.uint8)[..., 0] = 0
+    k[1, 0, 3] = 0.0
+    k[1, 0, 3, 0] = -448.0
+    v[1] = 0.0
+    v[1, 0, 3] = 448.0
+    k_scale = torch.full((pages, 1), 2.0 ** -3, device="cuda")
+    v_scale = torch.full((pages, 1), 2.0 ** -5, device="cuda")
+    v_scale[1] = 2.0 ** (loud - 5)
+    q = torch.randn((batch, heads, dim), generator=g, device="cuda")
+    q[:, :, 0] = 60.0 * dim ** 0.5 / 56.0  # the loud token's logit: -60
+    q = q.half()
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).expand(batch, pages).contiguous()
+    out = paged.attention_paged(q, paged.KVCache8(k, v, k_scale, v_scale), table, dev([n] * batch))
+    paged.check()
+    kn = k.double().reshape(-1, dim) * 2.0 ** -3
+    vn = (v.double() * v_scale.double()[:, :, None, None]).reshape(-1, dim)
+    quiet = vn.clone()
+    quiet[page + 3] = 0.0  # of weight e^-55 and less: not in the bound's largest value
+    rows, got = q.reshape(-1, dim), out.reshape(-1, dim)
+    for a in range(0, len(rows), 640):
+        worst = sink_error(got[a:a + 640], rows[a:a + 640], kn, quiet, "float16", 2.0 ** (loud - 30))
+        assert worst <= 1.0, worst
