@@ -33,9 +33,11 @@ class Layer(NamedTuple):
 
 
 class Stack:
-    """Attention layers of one Gemma expert's shape, with random weights."""
+    """Attention layers of one Gemma expert's shape, with random weights, for tokens at the first
+    ``positions`` positions."""
 
-    def __init__(self, cfg: GemmaExpertConfig, layers: int, vocab: int, dtype, seed: int, device="cuda"):
+    def __init__(self, cfg: GemmaExpertConfig, layers: int, vocab: int, dtype, seed: int, device="cuda",
+                 positions: int = 4096):
         g = torch.Generator(device=device).manual_seed(seed)
 
         def w(rows, cols):
@@ -47,8 +49,8 @@ class Stack:
         rows = (cfg.num_heads + 2 * cfg.num_kv_heads) * cfg.head_dim
         self.layers = [Layer(w(rows, cfg.width), w(cfg.width, cfg.num_heads * cfg.head_dim))
                        for _ in range(layers)]
-        cos, sin = make_rope_np(4096, cfg.head_dim, 10_000.0)
-        self.rope = [torch.as_tensor(np.asarray(x).reshape(4096, -1)).to(device) for x in (cos, sin)]
+        cos, sin = make_rope_np(positions, cfg.head_dim, 10_000.0)
+        self.rope = [torch.as_tensor(np.asarray(x).reshape(positions, -1)).to(device) for x in (cos, sin)]
 
     def project(self, layer: Layer, x: torch.Tensor, positions: torch.Tensor):
         """q, k and v of tokens at these positions: views of one projection, q and k rotated."""
@@ -73,7 +75,9 @@ class PagedSession:
 
     def __init__(self, stack: Stack, batch: int, most: int, page: int = 64):
         c = stack.cfg
-        self.stack, self.page = stack, page
+        if most > len(stack.rope[0]):
+            raise ValueError(f"requests of {most} tokens, a stack for {len(stack.rope[0])} positions")
+        self.stack, self.page, self.most, self.longest = stack, page, most, 0
         columns = -(-most // page)
         pages = batch * columns
         ints = dict(dtype=torch.int32, device=stack.device)
@@ -83,12 +87,16 @@ class PagedSession:
         self.caches = [paged.KVCache8.empty(pages, page, c.num_kv_heads, c.head_dim, stack.device)
                        for _ in stack.layers]
 
-    def _place(self, new: torch.Tensor, tokens: int) -> paged.Slots:
+    def _place(self, new: torch.Tensor, tokens: int, longest: int) -> paged.Slots:
+        """``longest``: the most new tokens of one request. Positions stay inside the stack's table."""
+        if self.longest + longest > self.most:
+            raise ValueError(f"a request may grow beyond the session's {self.most} tokens")
+        self.longest += longest
         return paged.build_slots(self.lens, new, self.table, self.free, self.pos, self.page, tokens)
 
     def prompts(self, x: torch.Tensor, new: torch.Tensor, prefix: torch.Tensor, longest: int):
         """Packed prompt embeddings [tokens, width] -> hidden states."""
-        s = self._place(new, len(x))
+        s = self._place(new, len(x), longest)
         for layer, cache in zip(self.stack.layers, self.caches):
             q, k, v = self.stack.project(layer, x, s.positions)
             x = self.stack.add(layer, x, paged.attention_prompt(q, k, v, s.cu_seqlens,
@@ -99,7 +107,7 @@ class PagedSession:
 
     def step(self, x: torch.Tensor):
         """One token per request, embeddings [batch, width] -> hidden states."""
-        s = self._place(torch.ones_like(self.lens), len(x))
+        s = self._place(torch.ones_like(self.lens), len(x), 1)
         for layer, cache in zip(self.stack.layers, self.caches):
             q, k, v = self.stack.project(layer, x, s.positions)
             paged.write_kv(cache, k, v, s.cu_seqlens, self.lens, s.slot_mapping, max_new=1)
@@ -124,7 +132,7 @@ def dense(stack: Stack, x: torch.Tensor, prefix: int) -> torch.Tensor:
 def run(cfg: GemmaExpertConfig, dtype: str = "float16", lens: List[int] = (70, 33, 129, 1),
         images: int = 32, steps: int = 12, layers: int = 2, vocab: int = 1000, seed: int = 0) -> bool:
     lens = list(lens)
-    stack = Stack(cfg, layers, vocab, getattr(torch, dtype), seed)
+    stack = Stack(cfg, layers, vocab, getattr(torch, dtype), seed, positions=max(lens) + steps)
     rng = np.random.default_rng(seed)
     prefix = [min(images, n) for n in lens]
     prompt = [torch.as_tensor(rng.integers(0, vocab, n).astype(np.int32)).cuda() for n in lens]
