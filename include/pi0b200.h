@@ -253,6 +253,7 @@ int pi0_write_kv(int dtype, const void* k, int64_t k_token_stride, int64_t k_hea
  * queries and Lk keys, query i sees key j if j ≤ i + Lk − Lq or j < prefix_lens[r] (NULL: 0,
  * causal; Lk: every query sees every key). out [total_q, heads, head_dim] = softmax(scale·q·kᵀ)·v
  * over the keys seen, fp32 softmax; a query that sees none, and a token of no request, give zeros.
+ * out may not overlap q, k or v, which are read while it is written.
  * Keys and values that a query does not see do not reach its result, whatever they hold. Head
  * sizes 64, 128 and 256 with up to 128 query heads per kv head run on tensor cores and need `err`,
  * which also takes the codes of bounded waits, and a workspace: 16-byte aligned, of the size that
@@ -271,7 +272,7 @@ int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64
 
 /* Attention of one token per request over the cache: q, out [batch, heads, head_dim]; the request
  * sees its kv_lens[r] cached tokens (the new one's keys and values are written before the call).
- * A request without any gives zeros. workspace (16-byte aligned, of the size that
+ * A request without any gives zeros. out may be q, with its strides. workspace (16-byte aligned, of the size that
  * pi0_attention_paged_workspace returns for the current device; -1: bad sizes or no device) holds
  * what the parts of a request's tokens add up to until they are joined: its contents before and
  * after a call do not matter, but calls that may run at the same time need one each. Head sizes 64,

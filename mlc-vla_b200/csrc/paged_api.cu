@@ -35,6 +35,20 @@ bool rows_ok(const void* p, int64_t tok, int64_t head) {
   return p && !off16(p) && tok > 0 && head > 0 && tok % 8 == 0 && head % 8 == 0;
 }
 
+// whether two operands [tokens, heads, head_dim] surely share elements: they begin at the same one, or
+// both are contiguous and their ranges meet (others may lie between one another's rows)
+struct Operand {
+  const void* p;
+  int64_t tokens, heads, head_dim, tok, head;
+  bool dense() const { return tok == heads * head_dim && head == head_dim; }
+  bool meets(const Operand& o) const {
+    if (tokens == 0 || o.tokens == 0) return false;
+    if (p == o.p) return true;
+    const auto *x = static_cast<const uint16_t*>(p), *y = static_cast<const uint16_t*>(o.p);
+    return dense() && o.dense() && x < y + o.tokens * o.tok && y < x + tokens * tok;
+  }
+};
+
 bool cache_ok(const pi0_kv8* c) {
   return c && c->k && c->v && c->k_scale && c->v_scale && !off16(c->k) && !off16(c->v) &&
          c->num_pages >= 1 && c->page_size >= 1 && c->kv_heads >= 1 && c->head_dim >= 8 &&
@@ -349,6 +363,12 @@ int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64
     return PI0_ERR_INVALID;
   const int64_t rows = (int64_t)total_q * heads;
   if (rows > INT_MAX) return PI0_ERR_UNSUPPORTED;
+  // queries, keys and values are read again after rows have been written
+  const Operand o{out, total_q, heads, head_dim, o_token_stride, o_head_stride};
+  if (o.meets({q, total_q, heads, head_dim, q_token_stride, q_head_stride}) ||
+      o.meets({k, total_k, kv_heads, head_dim, k_token_stride, k_head_stride}) ||
+      o.meets({v, total_k, kv_heads, head_dim, v_token_stride, v_head_stride}))
+    return PI0_ERR_INVALID;
   PromptArgs a{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
                v_token_stride, v_head_stride, o_token_stride, o_head_stride, cu_seqlens_q,
                cu_seqlens_k, prefix_lens, err, static_cast<float*>(workspace),

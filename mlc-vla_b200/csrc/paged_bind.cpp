@@ -2,6 +2,7 @@
 // workspaces and error flags, and the calls of the C entry points of include/pi0b200.h. A decode
 // step makes these calls once per layer and token; from Python the checks alone took 11 us a call,
 // longer than the kernels.
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -275,6 +276,13 @@ Tensor attention_prompt(const Tensor& q, const Tensor& k, const Tensor& v, const
   Tensor o = out ? *out : at::empty(q.sizes(), q.options());
   const Rows orr = rows(o, "out", dev, type);
   check_shape(o, "out", q.sizes());
+  if (out && tokens > 0)
+    for (const Tensor* t : {&q, &k, &v}) {
+      const auto s = at::get_overlap_status(o, *t);
+      TORCH_CHECK_VALUE((t->numel() == 0 || o.data_ptr() != t->data_ptr()) &&
+                            s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial,
+                        "out may not overlap q, k or v");
+    }
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
   const int64_t bytes = g_lib.attention_prompt_workspace(fits32(heads, "heads"), (int)kv_heads, (int)dim);
   if (bytes < 0) throw Status(PI0_ERR_CUDA, "pi0_attention_prompt_workspace");

@@ -115,7 +115,7 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``cu_seqlens_k[r]:cu_seqlens_k[r + 1]`` (default: the same), the last query at the last key.
     Query i of Lq sees key j of Lk if ``j <= i + Lk - Lq`` or ``j < prefix_lens[r]`` (default 0:
     causal; Lk: every key). ``scale``: of the logits, 1/sqrt(head_dim) by default. A query that
-    sees no key gives zeros."""
+    sees no key gives zeros. ``out``: for the result, apart from q, k and v."""
     return _native().attention_prompt(q, k, v, cu_seqlens_q, cu_seqlens_k, prefix_lens, scale, out,
                                       err)
 
@@ -126,7 +126,7 @@ def attention_paged(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor,
                     err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one token per request, q [batch, heads, head_dim], over its ``kv_lens[r]``
     tokens in the pages ``block_table[r]`` of ``cache`` (its own among them: ``write_kv`` goes
-    before). A request without any gives zeros."""
+    before). A request without any gives zeros. ``out``: for the result; it may be q."""
     return _native().attention_paged(q, *cache, block_table, kv_lens, scale, out, err)
 
 

@@ -474,3 +474,32 @@ def test_paged_loud_page(heads, dim, page, loud):
     for a in range(0, len(rows), 640):
         worst = sink_error(got[a:a + 640], rows[a:a + 640], kn, quiet, "float16", 2.0 ** (loud - 30))
         assert worst <= 1.0, worst
+
+
+# ---- outputs and gradients --------------------------------------------------------------------------
+
+def test_out_apart_from_the_inputs():
+    from mlc_vla import paged
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    fused = torch.randn((300, 20, 64), generator=g, device="cuda").half()
+    q, k, v, room = fused[:, :8], fused[:, 8:10], fused[:, 10:12], fused[:, 12:]
+    cu = dev([0, 100, 300])
+    want = paged.attention_prompt(q, k, v, cu)
+    paged.attention_prompt(q, k, v, cu, out=room)  # between the rows of its inputs
+    assert torch.equal(room, want)
+    dense = torch.randn((301, 8, 64), generator=g, device="cuda").half()
+    for out, query in ((q, q), (dense[1:], dense[:300]), (dense[:300], dense[1:])):
+        with pytest.raises(ValueError, match="overlap"):
+            paged.attention_prompt(query, k, v, cu, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        paged.attention_prompt(q, dense[:300], dense[:300].clone(), cu, out=dense[:300])
+    # over the cache the result may replace the queries
+    rng = np.random.default_rng(0)
+    for dim in (64, 72):
+        lens = [3000, 1, 700]
+        c, table = filled_cache(rng, lens, 16, 2, dim)
+        x = torch.randn((3, 8, dim), generator=g, device="cuda").half()
+        want = paged.attention_paged(x, c, dev(table), dev(lens))
+        assert torch.equal(paged.attention_paged(x, c, dev(table), dev(lens), out=x), want)
+        paged.check()

@@ -61,3 +61,20 @@ def test_compare_paged_rotates_every_position_that_it_reaches():
         session.step(x[:2])
     with pytest.raises(ValueError, match="beyond the session's 40"):
         PagedSession(stack, 2, 40).prompts(x, torch.tensor([1, 2]), torch.tensor([0, 0]), 41)
+
+
+def test_attention_prompt_refuses_out_over_its_inputs():
+    from mlc_vla import _lib
+
+    lib = _lib.load()
+
+    def call(out, tok=512, k_tok=128, total=4):
+        p = ctypes.c_void_p
+        return lib.pi0_attention_prompt(1, p(1 << 20), tok, 64, p(2 << 20), k_tok, 64, p(3 << 20), k_tok,
+                                        64, total, total, 8, 2, 64, 1, p(4096), p(4096), None, 0.125,
+                                        p(out), tok, 64, None, 0, None, None)
+
+    for out in (1 << 20, 2 << 20, 3 << 20, (1 << 20) + 1024, (1 << 20) - 1024, (3 << 20) + 1008,
+                (2 << 20) - 4 * 1024 + 16):
+        assert call(out) == _lib.PI0_ERR_INVALID
+    assert call(1 << 20, tok=1024) == _lib.PI0_ERR_INVALID
