@@ -5,6 +5,8 @@
 #include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <map>
@@ -178,6 +180,29 @@ int* err_of(const OptTensor& err, int device) {
   return static_cast<int*>(flag_of(device).data_ptr());
 }
 
+// The attentions have no backward pass. A result of inputs that ask for gradients says so when one is
+// asked of it, rather than being a constant without a word.
+bool wants_grad(std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : inputs)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+void no_grad_out(const OptTensor& out, bool wanted) {
+  TORCH_CHECK(!(out && (wanted || wants_grad({&*out}))),
+              "out= does not support gradients: call under torch.no_grad()");
+}
+
+void no_backward(Tensor& o, const char* name, std::initializer_list<const Tensor*> inputs) {
+  torch::autograd::edge_list edges;
+  for (const Tensor* t : inputs)
+    if (t->requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+  auto node = std::shared_ptr<torch::autograd::NotImplemented>(
+      new torch::autograd::NotImplemented(name, std::move(edges)), torch::autograd::deleteNode);
+  torch::autograd::set_history(o, node);
+}
+
 // n elements of a one-dimensional tensor from `first` on, without the dispatcher's way around
 Tensor part_of(const Tensor& t, int64_t first, int64_t n) {
   Tensor v = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(),
@@ -273,6 +298,8 @@ Tensor attention_prompt(const Tensor& q, const Tensor& k, const Tensor& v, const
   c10::cuda::OptionalCUDAGuard guard;
   if (c10::cuda::current_device() != dev) guard.set_index(dev);
   at::AutoDispatchBelowAutograd below;
+  const bool grad = wants_grad({&q, &k, &v});
+  no_grad_out(out, grad);
   Tensor o = out ? *out : at::empty(q.sizes(), q.options());
   const Rows orr = rows(o, "out", dev, type);
   check_shape(o, "out", q.sizes());
@@ -295,6 +322,7 @@ Tensor attention_prompt(const Tensor& q, const Tensor& k, const Tensor& v, const
                                       orr.tok, orr.head, ws.data_ptr(), ws.numel(),
                                       err_of(err, dev), stream),
                "pi0_attention_prompt");
+  if (grad) no_backward(o, "attention_prompt", {&q, &k, &v});
   return o;
 }
 
@@ -316,6 +344,8 @@ Tensor attention_paged(const Tensor& q, const Tensor& ck, const Tensor& cv, cons
   c10::cuda::OptionalCUDAGuard guard;
   if (c10::cuda::current_device() != dev) guard.set_index(dev);
   at::AutoDispatchBelowAutograd below;
+  const bool grad = wants_grad({&q, &cks, &cvs});
+  no_grad_out(out, grad);
   Tensor o = out ? *out : at::empty(q.sizes(), q.options());
   const Rows orr = rows(o, "out", dev, q.scalar_type());
   check_shape(o, "out", q.sizes());
@@ -332,6 +362,7 @@ Tensor attention_paged(const Tensor& q, const Tensor& ck, const Tensor& cv, cons
                                      orr.p, orr.tok, orr.head, ws.data_ptr(), ws.numel(),
                                      err_of(err, dev), stream),
                "pi0_attention_paged");
+  if (grad) no_backward(o, "attention_paged", {&q, &cks, &cvs});
   return o;
 }
 

@@ -14,6 +14,9 @@ Every call is asynchronous on the current stream of its tensors' device. What on
 see (a negative length, an exhausted pool, a page number outside the pool) is recorded in `err`, a
 device int32 tensor of one element, or, where none is given, in a flag of the device that
 ``check()`` reads, clears and raises.
+
+There is no backward pass: an attention of tensors that ask for gradients gives a result whose
+backward raises, and what ``write_kv`` stores has no history.
 """
 
 from __future__ import annotations

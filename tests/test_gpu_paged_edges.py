@@ -503,3 +503,35 @@ def test_out_apart_from_the_inputs():
         want = paged.attention_paged(x, c, dev(table), dev(lens))
         assert torch.equal(paged.attention_paged(x, c, dev(table), dev(lens), out=x), want)
         paged.check()
+
+
+def test_gradients_are_refused_where_they_are_asked_for():
+    from mlc_vla import paged
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn((20, h, 64), generator=g, device="cuda").half() for h in (4, 2, 2))
+    cu = dev([0, 20])
+    rng = np.random.default_rng(0)
+    c, table = filled_cache(rng, [50] * 20, 16, 2, 64)
+    calls = [lambda q, k, v, **kw: paged.attention_prompt(q, k, v, cu, **kw),
+             lambda q, k, v, **kw: paged.attention_paged(q, c, dev(table), dev([50] * 20), **kw)]
+    for call in calls:
+        want = call(q, k, v)
+        assert not want.requires_grad
+        weight = torch.ones((), device="cuda", dtype=torch.float16, requires_grad=True)
+        out = call(q * weight, k, v)
+        assert torch.equal(out, want)  # forward as ever
+        with pytest.raises(RuntimeError, match="not implemented"):
+            out.float().sum().backward()
+        room = torch.empty_like(q)
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call(q * weight, k, v, out=room)
+        with torch.no_grad():
+            assert not call(q * weight, k, v).requires_grad
+            call(q * weight, k, v, out=room)
+        assert torch.equal(room, want)
+    out = calls[0](q, k, v.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="not implemented"):
+        out.float().sum().backward()
+    with torch.inference_mode():
+        assert torch.equal(calls[0](q, k, v), calls[0](q.clone(), k, v))
