@@ -11,7 +11,6 @@
 
 #include <map>
 #include <mutex>
-#include <utility>
 #include <vector>
 
 #include "pi0b200.h"
@@ -58,7 +57,6 @@ void check_status(int rc, const char* name) {
 // Never freed: a static destructor would run after CUDA is gone.
 std::mutex g_mutex;
 auto& g_flags = *new std::map<int, Tensor>;
-auto& g_workspaces = *new std::map<std::pair<int, cudaStream_t>, Tensor>;
 
 bool capturing(cudaStream_t stream) {
   cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
@@ -87,15 +85,9 @@ OptTensor flag(int device) {
   return it == g_flags.end() ? OptTensor() : OptTensor(it->second);
 }
 
-// Room for the partial sums of one call. Calls on one stream follow each other, so a stream's calls
-// share a buffer; a captured graph may be replayed on any stream and has its own.
-Tensor workspace(int device, cudaStream_t stream, int64_t bytes) {
-  const auto options = at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device);
-  if (capturing(stream)) return at::empty({bytes}, options);
-  std::lock_guard<std::mutex> lock(g_mutex);
-  Tensor& t = g_workspaces[{device, stream}];
-  if (!t.defined() || t.numel() < bytes) t = at::empty({bytes}, options);
-  return t;
+// Room for the partial sums of one call, from the stream's pool and back to it.
+Tensor workspace(int device, int64_t bytes) {
+  return at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
 }
 
 int dtype_code(const Tensor& t, const char* name) {
@@ -313,7 +305,7 @@ Tensor attention_prompt(const Tensor& q, const Tensor& k, const Tensor& v, const
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
   const int64_t bytes = g_lib.attention_prompt_workspace(fits32(heads, "heads"), (int)kv_heads, (int)dim);
   if (bytes < 0) throw Status(PI0_ERR_CUDA, "pi0_attention_prompt_workspace");
-  const Tensor ws = workspace(dev, stream, bytes);
+  const Tensor ws = workspace(dev, bytes);
   check_status(g_lib.attention_prompt(code, qr.p, qr.tok, qr.head, kr.p, kr.tok, kr.head, vr.p,
                                       vr.tok, vr.head, fits32(tokens, "tokens"),
                                       fits32(k.size(0), "keys"), fits32(heads, "heads"),
@@ -353,7 +345,7 @@ Tensor attention_paged(const Tensor& q, const Tensor& ck, const Tensor& cv, cons
   const int64_t bytes = g_lib.attention_paged_workspace(fits32(heads, "heads"), c.kv_heads,
                                                         c.head_dim, c.page_size);
   if (bytes < 0) throw Status(PI0_ERR_CUDA, "pi0_attention_paged_workspace");
-  const Tensor ws = workspace(dev, stream, bytes);
+  const Tensor ws = workspace(dev, bytes);
   check_status(g_lib.attention_paged(code, qr.p, qr.tok, qr.head, fits32(batch, "requests"),
                                      (int)heads, &c, table,
                                      batch < 2 ? columns : block_table.stride(0),

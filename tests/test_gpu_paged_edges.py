@@ -535,3 +535,27 @@ def test_gradients_are_refused_where_they_are_asked_for():
         out.float().sum().backward()
     with torch.inference_mode():
         assert torch.equal(calls[0](q, k, v), calls[0](q.clone(), k, v))
+
+
+def test_calls_keep_no_memory():
+    """Workspaces return to the allocator, whatever streams the calls were on."""
+    from mlc_vla import paged
+
+    rng = np.random.default_rng(0)
+    c, table = filled_cache(rng, [3000, 10], 16, 1, 256)
+    x = torch.randn((200, 8, 256), device="cuda").half()
+    args = (x[:2], c, dev(table), dev([3000, 10]))
+    cu = dev([0, 200])
+    want = paged.attention_paged(*args), paged.attention_prompt(x, x[:, :1], x[:, 1:2], cu)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(4):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got = paged.attention_paged(*args), paged.attention_prompt(x, x[:, :1], x[:, 1:2], cu)
+        s.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del got
+    assert torch.cuda.memory_allocated() == before
+    paged.check()
