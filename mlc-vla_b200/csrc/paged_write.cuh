@@ -134,6 +134,9 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
     const int nv = n * vec, dt = lanes / vec, dd = lanes % vec;
     const int64_t tok_stride = a.tok_stride[kind];
     auto at = [&](int v) { return src + (v / vec) * tok_stride + (v % vec) * 8; };
+    const int* slots = a.slots + tok;
+    int slot0 = slots[0];  // of the run's first token
+    const int mine = g < n ? slots[g] : slot0 + g;
     uint4 held[VECS];
     {
       int d = g % vec;
@@ -152,14 +155,12 @@ __global__ void __launch_bounds__(32 * kWriteWarps, VECS > 4 ? 2 : 4) write_kv_k
     }
     // Every token at its row of one page, which is the first's: looked at while the vectors are on
     // their way. If not, the unit takes the path of infinities, which looks at each token.
-    const int* slots = a.slots + tok;
     const int pool = c.num_pages * ps;
-    int slot0 = slots[0];  // of the run's first token
-    bool odd = (unsigned)slot0 >= (unsigned)pool || slot0 % ps != row;
+    bool odd = (unsigned)slot0 >= (unsigned)pool || slot0 % ps != row || mine != slot0 + g;
     float* scales = kind ? c.vs : c.ks;
     auto scale_at = [&]() { return scales + (int64_t)(slot0 / ps) * c.kv_heads + h; };
     float old = row > 0 && !odd ? *scale_at() : 0.f;
-    for (int i = g; i < n; i += lanes) odd |= slots[i] != slot0 + i;
+    for (int i = g + lanes; i < n; i += lanes) odd |= slots[i] != slot0 + i;
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) m = max_bits<T>(m, held[i]);
