@@ -196,8 +196,9 @@ int pi0_vision_profile_read(pi0_vision_ctx* ctx, int n_families, int64_t* launch
  * maps from request lengths, new tokens into the cache, attention of packed prompts, attention of
  * one token per request over the cache. All context-free, all buffers the caller's, all int32
  * arrays on the device. `err` (a device int, may be NULL) takes the first of pi0_paged_err and
- * pi0_device_error's codes that a call meets and is left alone otherwise; what such a call wrote
- * stays inside its buffers, and requests without a fault have their results.
+ * pi0_device_error's codes that a call meets and is left alone otherwise, also by calls that find
+ * one there; what such a call wrote stays inside its buffers, and requests without a fault have their
+ * results (all of a call's are undefined after the code of a bounded wait).
  *
  * A page holds page_size tokens of one request. Token `pos` of request r lies in page
  * block_table[r, pos / page_size] at row pos % page_size; its slot is page·page_size + row. */
@@ -272,12 +273,12 @@ int pi0_attention_prompt(int dtype, const void* q, int64_t q_token_stride, int64
 
 /* Attention of one token per request over the cache: q, out [batch, heads, head_dim]; the request
  * sees its kv_lens[r] cached tokens (the new one's keys and values are written before the call).
- * A request without any gives zeros. out may be q, with its strides. workspace (16-byte aligned, of the size that
- * pi0_attention_paged_workspace returns for the current device; -1: bad sizes or no device) holds
- * what the parts of a request's tokens add up to until they are joined: its contents before and
- * after a call do not matter, but calls that may run at the same time need one each. Head sizes 64,
- * 128 and 256 on pages of 8, 16, 32 or 64 tokens or of whole 128s run on tensor cores and need
- * `err`, which also takes the codes of bounded waits; the others need neither. */
+ * A request without any gives zeros. out may be q, with its strides. workspace (16-byte aligned, of
+ * the size that pi0_attention_paged_workspace returns for the current device; -1: bad sizes or no
+ * device) holds what the parts of a request's tokens add up to until they are joined: its contents
+ * before and after a call do not matter, but calls that may run at the same time need one each. Head
+ * sizes 64, 128 and 256 on pages of 8, 16, 32 or 64 tokens or of whole 128s run on tensor cores and
+ * need `err`, which also takes the codes of bounded waits; the others need neither. */
 int64_t pi0_attention_paged_workspace(int heads, int kv_heads, int head_dim, int page_size);
 int pi0_attention_paged(int dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                         int batch, int heads, const pi0_kv8* cache, const int32_t* block_table,

@@ -22,10 +22,10 @@
 // Bound by HBM: 2 bytes per key, kv head and dimension. Per tile of 128 keys and 256 dimensions
 // (64 KB, 1.5 µs of one SM's share of HBM) the MMAs are 16 instructions of N = 32 and the softmax
 // 8 exponentials a thread, so one warpgroup hides behind the loads; narrower heads load faster and
-// get two or three CTAs per SM. Measured: 64 requests of 8192 tokens, 32 heads on 8 of 128, 171 us in
-// pages of 128 (6260 GB/s, 96 % of the measured copy rate) and 180 us in pages of 16; of lengths 1 to
-// 16384, 182 us (5970 GB/s). Short requests are bound by latency: one of 1005 tokens takes 10 us,
-// 32 of 700 to 1100 14 us.
+// get two or three CTAs per SM. Measured: 64 requests of 8192 tokens, 32 heads on 8 of 128, 169 us in
+// pages of 128 (6380 GB/s, 97 % of the measured copy rate) and 181 us in pages of 16; of lengths 1 to
+// 16384, 186 us (5850 GB/s). Groups of 8 heads 204 us, of 16 395 us: there the softmax bounds it. Short
+// requests are bound by latency: one of 1005 tokens takes 9.8 us, 32 of 700 to 1100 14.8 us.
 //
 // Work split: the tiles of all (request, kv head) units are numbered in one row and every CTA takes
 // an equal, contiguous share, whatever the lengths are; when that is only a few tiles, as many CTAs as
@@ -102,7 +102,9 @@ __device__ __forceinline__ int readable_len(const DecodeArgs& a, int b) {
   return n;
 }
 
-// One warp per (request, head), for the head and page sizes without a tensor-core form.
+// One warp per (request, head), for the head and page sizes without a tensor-core form: a key at a time,
+// 0.8 us each. 32 requests of 900 tokens take 710 us in pages of 24 or 48 (16 us in pages of 64), one
+// of 16384 tokens with heads of 96 12.9 ms.
 template <typename T>
 __global__ void __launch_bounds__(32) paged_rows_kernel(DecodeArgs a) {
   const int b = blockIdx.y, h = blockIdx.x;

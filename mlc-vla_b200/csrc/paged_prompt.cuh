@@ -4,7 +4,7 @@
 // n(i) = min(Lk, max(i + Lk − Lq + 1, prefix)): always a leading part of the request's keys. A row is
 //   o = Σ_j 2^(c·q·k_j − m) v_j / Σ_j 2^(c·q·k_j − m),   c = scale·log2 e,
 // in one pass over the keys with a running reference m that is raised, and the sums rescaled, only
-// when a row's maximum outgrows it by 2^8.
+// when a row's maximum outgrows it by 2^8 (kLift).
 //
 // Tensor-core form (head sizes 64, 128, 256). A tile of query rows is the group's heads of as many
 // tokens as fit into 128 rows, so heads that share keys share their loads, and a tile of one kv head
@@ -21,13 +21,14 @@
 // 3600 clocks for two tiles (2048 of products): from logits to logits a tile spends 600 on loading them
 // and their maximum, 1450 in its exponentials, 1100 in P·V and the next logits, whose reads of shared
 // memory compete with the loads of K and V, and the rest on handing over; power lowers the clock.
-// Measured: 8192 tokens, 32 heads on 8 of 128, all keys 828 us (1327 TFLOP/s, 80 % of the measured
-// 1661), causal 475 us (1156); 8 heads on 1 of 256, all keys 401 us (1370).
+// Measured: 8192 tokens, 32 heads on 8 of 128, all keys 849 us (1295 TFLOP/s, 78 % of the measured
+// 1661), causal 480 us (1145); 8 heads on 1 of 256, all keys 404 us (1360); 32 heads on 8 of 64, all
+// keys 740 us (740), where the exponentials alone are 500 us at the clock that it runs at.
 //
 // Work split: the steps of all (tile, kv head) are numbered in one row, and every CTA takes an equal,
 // contiguous share, whatever the lengths are. What lies in several CTAs leaves partial sums that a
 // second kernel joins in the order of the CTAs: eight chunks of up to 300 tokens on 1000 to 4000
-// earlier keys take 58 us instead of 85 with a CTA per tile.
+// earlier keys take 59 us instead of 85 with a CTA per tile.
 #pragma once
 
 #include <type_traits>
@@ -80,7 +81,8 @@ struct PromptKV {
 constexpr int kRowWarps = 4;
 
 // One warp per (token, head), for the head sizes without a tensor-core form and scales that are not
-// positive.
+// positive: 3 TFLOP/s with heads of 96 (8 prompts of 900 tokens and 8 heads 2.8 ms, against 0.04 ms with
+// heads of 128), 8 with heads of 256.
 template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) prompt_rows_kernel(PromptArgs a) {
   const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
@@ -800,8 +802,8 @@ __global__ void __launch_bounds__(PromptCfg<HD>::THREADS, 1)
         if (ok) ok = bar_wait(&pv_done[last & 1], (last >> 1) & 1, waits, tc::ERR_TIMEOUT_EPI);
         ok = __all_sync(~0u, ok);
         tc_fence_after();
-        // o = O / l, or O as it is for the joining kernel. A row that sees no key is zero, and one of
-        // a kernel that gave up waiting NaN.
+        // o = O / l, or O as it is for the joining kernel. A row that sees no key is zero, and one
+        // whose products were not waited for to the end NaN.
         const float inv = !ok ? NAN : whole ? 1.f / l : 1.f;
         const uint64_t inv2 = pack2(inv, inv);
         uint64_t nan2[2] = {0, 0};  // sums of 0·o: NaN once an element is no number

@@ -12,10 +12,11 @@
 // Bound by HBM: 2 bytes read and 1 written per element, plus the scales. A (page, kv head) is held in
 // the registers of the few warps that take it, up to 16 vectors of 16 bytes a lane: one pass over the
 // data, whose loads are all in flight before the first is used, and no wait but one between those
-// warps. Larger pages are read twice. Measured: 32771 tokens of 8 heads of 128 in pages of 32, 39 us
-// (5190 GB/s, 79 % of the measured copy rate); 16 vectors a lane in two blocks per SM, against 53 us
+// warps. Larger pages are read twice. Measured: 32771 tokens of 8 heads of 128 in pages of 32, 39.0 us
+// (5166 GB/s, 79 % of the measured copy rate); 16 vectors a lane in two blocks per SM, against 53 us
 // with 8 in three and 62 us with 4 in four: what counts is the bytes in flight. 256 single tokens
-// 4.6 us, bound by latency.
+// 4.7 us, bound by latency. The launch has blocks for every request's longest: one prompt of 8192
+// beside 256 single tokens takes 595 us for 8 us of bytes, so such batches are better written apart.
 #pragma once
 
 #include "paged_common.cuh"
